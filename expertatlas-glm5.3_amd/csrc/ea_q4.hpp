@@ -1,0 +1,113 @@
+// Products with 4-bit weights in groups: W[n, k] = s q + b with q in 0..15 and one (s, b) a row and group of 32, 64 or 128
+// consecutive k. A sum over a group is s (sum of q x) + b (sum of x), so the integers q go into the matrix instructions as
+// they are (exact in 16 bits) and s and b act on fp32 sums once a group: no weight is ever rounded.
+//
+// Layout (ea_q4_pack): a matrix [N, K] is cut into tiles of 16 rows (the last filled up with zeros) and chunks of 128 k
+// (likewise); a tile's chunk is 1024 bytes of words, then 16 rows x 128 / group words (s in the low half, b in the high).
+// Lane l of a wave reads the 16 bytes at 16 l of the words: word j holds row l & 15 at k = 32 j + 8 (l >> 4) + 0..7, the B
+// operand of the chunk's j-th 16x16x32 product; so a wave's read of a chunk is one contiguous kilobyte. In a word, k + 0..3
+// are in the even half-bytes and k + 4..7 in the odd ones: masked by 0x0f0f0f0f, four of them are four bytes q, and a byte
+// q < 16 read as e4m3 is q / 512 exactly (below 8 a subnormal), which one conversion with the scale 512 turns into q.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include "ea_device.hpp"
+
+namespace ea {
+
+typedef __bf16 b8v __attribute__((ext_vector_type(8)));
+typedef u4v u4v_a8 __attribute__((aligned(8)));  // 16 bytes of a row of activations, rows 8-byte aligned
+
+constexpr int Q4_CHUNK = 128, Q4_WORDS = 1024;
+
+// gpc: groups a chunk (4, 2 or 1 for groups of 32, 64, 128)
+__host__ __device__ constexpr int q4_chunk_bytes(int gpc) { return Q4_WORDS + 64 * gpc; }
+__host__ __device__ inline uint32_t q4_chunks(uint32_t k) { return k / Q4_CHUNK + (k % Q4_CHUNK != 0); }
+__host__ __device__ inline uint32_t q4_tiles(uint32_t n) { return n / 16 + (n % 16 != 0); }
+
+template <bool BF>
+__device__ __forceinline__ f4v q4_mfma(const u4v& a, const u4v& b, const f4v& c) {
+    if constexpr (BF)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8v, a), __builtin_bit_cast(b8v, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8v, a), __builtin_bit_cast(h8v, b), c, 0, 0, 0);
+}
+
+// The eight values of a word as bf16 or fp16 integers.
+template <bool BF>
+__device__ __forceinline__ u4v q4_values(uint32_t w) {
+    const uint32_t lo = w & 0x0f0f0f0fu, hi = (w >> 4) & 0x0f0f0f0fu;
+    if constexpr (BF)
+        return u4v{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 512.0f, false)),
+                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 512.0f, true)),
+                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 512.0f, false)),
+                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 512.0f, true))};
+    else
+        return u4v{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 512.0f, false)),
+                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 512.0f, true)),
+                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 512.0f, false)),
+                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 512.0f, true))};
+}
+
+template <bool BF>
+__device__ __forceinline__ u4v q4_ones() {
+    constexpr uint32_t one = BF ? 0x3f803f80u : 0x3c003c00u;
+    return u4v{one, one, one, one};
+}
+
+// A chunk's (s, b) of the lane's weight row.
+template <int GPC>
+struct Q4Params {
+    uint32_t w[GPC];
+};
+template <int GPC>
+__device__ __forceinline__ Q4Params<GPC> q4_params(const uint8_t* chunk, int lane) {
+    return *reinterpret_cast<const Q4Params<GPC>*>(chunk + Q4_WORDS + 4 * GPC * (lane & 15));
+}
+__device__ __forceinline__ void q4_scale_bias(uint32_t p, bool bf, float& s, float& b) {
+    s = bf ? __builtin_bit_cast(float, p << 16) : h2f((uint16_t)(p & 0xffffu));
+    b = bf ? __builtin_bit_cast(float, p & 0xffff0000u) : h2f((uint16_t)(p >> 16));
+}
+
+// One chunk of one tile against MT groups of 16 rows: out += the chunk's share. a[mt][j]: the rows' A operands of the
+// chunk's four products. The sums of x come from the same operands against ones, which leaves them in the accumulators'
+// own layout. D layout: lane l holds row 4 (l >> 4) + i, weight row l & 15.
+template <bool BF, int GPC, int MT>
+__device__ __forceinline__ void q4_chunk(const u4v& words, const Q4Params<GPC>& par, const u4v (&a)[MT][4], bool sbf,
+                                         f4v (&out)[MT]) {
+    constexpr int JPG = 4 / GPC;
+#pragma unroll
+    for (int g = 0; g < GPC; ++g) {
+        f4v acc[MT], xs[MT];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) acc[mt] = xs[mt] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < JPG; ++j) {
+            const u4v b = q4_values<BF>(words[g * JPG + j]);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                acc[mt] = q4_mfma<BF>(a[mt][g * JPG + j], b, acc[mt]);
+                xs[mt] = q4_mfma<BF>(a[mt][g * JPG + j], q4_ones<BF>(), xs[mt]);
+            }
+        }
+        float s, b;
+        q4_scale_bias(par.w[g], sbf, s, b);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                out[mt][i] = __builtin_fmaf(b, xs[mt][i], __builtin_fmaf(s, acc[mt][i], out[mt][i]));
+    }
+}
+
+// The lane's A operands of one chunk of a row of 16-bit activations; zeros from k on (k a multiple of 32).
+__device__ __forceinline__ void q4_rows(const uint16_t* row, uint32_t chunk, uint32_t k, int lane, u4v (&a)[4]) {
+    const uint16_t* p = row + (size_t)chunk * Q4_CHUNK + 8 * (lane >> 4);
+    const int left = (int)(k - chunk * Q4_CHUNK);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        a[j] = 32 * j < left ? (u4v) * reinterpret_cast<const u4v_a8*>(p + 32 * j) : u4v{0, 0, 0, 0};
+}
+
+}  // namespace ea

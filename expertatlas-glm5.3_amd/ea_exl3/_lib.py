@@ -74,6 +74,20 @@ class SwapStats(C.Structure):
     _fields_ = [("experts", U32), ("up", U32), ("down", U32), ("read_bytes", U64)]
 
 
+class Q4Linear(C.Structure):
+    _fields_ = [("words", U64), ("k", U32), ("n", U32), ("group", U32), ("s_dtype", I32)]
+
+
+class Q4Experts(C.Structure):
+    _fields_ = [("gu", U64), ("down", U64), ("count", U32), ("dims", U32), ("width", U32), ("group", U32),
+                ("s_dtype", I32), ("reserved", U32)]
+
+
+class Q4Scratch(C.Structure):
+    _fields_ = [("sorted", U64), ("items", U64), ("count", U64), ("h", U64), ("y", U64), ("rows", U32), ("slots", U32),
+                ("experts", U32), ("dims", U32), ("width", U32), ("reserved", U32)]
+
+
 assert C.sizeof(Job) == 88 and C.sizeof(Jobs) == 272 and C.sizeof(RotJobs) == 48  # exl3.zig:30-32
 
 # name -> (restype, argtypes); every entry point of include/ea_exl3.h
@@ -107,6 +121,13 @@ SIGNATURES = {
     "ea_linear_call_rotated": (I32, [P, C.POINTER(LinearScratch), P, U32, U32, P, P]),
     "ea_topk8": (I32, [P, P, P, P, P, U32, F32, P]),
     "ea_router": (I32, [P, P, I32, U32, P, P, P, U32, U32, U32]),
+    "ea_route": (I32, [P, P, I32, U32, P, P, P, U32, U32, U32, I32, U32, U32, U32, I32, F32]),
+    "ea_q4_bytes": (C.c_size_t, [U32, U32, U32]),
+    "ea_q4_pack": (I32, [P, P, P, P, P, P, P, P, U32, U32, U32, I32, U32]),
+    "ea_q4_call": (I32, [P, P, U32, P, I32, U32, U32, P, P]),
+    "ea_q4_scratch_bytes": (C.c_size_t, [C.POINTER(Q4Experts), U32, U32]),
+    "ea_q4_scratch_init": (I32, [C.POINTER(Q4Scratch), P, C.c_size_t, C.POINTER(Q4Experts), U32, U32]),
+    "ea_q4_routed": (I32, [P, P, I32, U32, P, P, C.POINTER(Q4Experts), C.POINTER(Q4Scratch), P, I32, U32]),
     "ea_swiglu2": (I32, [P, P, P, P, U32, U32]),
     "ea_add_f32": (I32, [P, P, P, C.c_size_t]),
     "ea_bank_open": (I32, [C.c_char_p, U32, U32, U32, C.POINTER(P)]),

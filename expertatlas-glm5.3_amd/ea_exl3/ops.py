@@ -1,5 +1,5 @@
-"""The routing input and the shared expert's activation: ops.router (ops.zig:131-136), ops.topk (ops.zig:187-191)
-and swiglu2 (native_ops.cu)."""
+"""The routing input and the shared expert's activation: ops.router (ops.zig:131-136), ops.topk (ops.zig:187-191), route
+(topk for other routers) and swiglu2 (native_ops.cu)."""
 from __future__ import annotations
 
 from ._lib import check, lib
@@ -15,6 +15,20 @@ def router(stream: int, x: int, x_stride: int, w: int, part: int, out: int, m: i
 def topk(stream: int, logits: int, bias: int, pick: int, wts: int, rows: int, scale: float = 2.5, log: int = 0) -> None:
     """pick int32 / wts fp32 [rows, 8]: sigmoid + bias, top 8 (lower id on ties), wts normalised * scale."""
     check(lib().ea_topk8(stream, logits, bias, pick, wts, rows, scale, log), "topk")
+
+
+SIGMOID, SOFTMAX = 0, 1
+
+
+def route(stream: int, logits: int, l_dtype: int, l_stride: int, bias: int, pick: int, wts: int, rows: int, experts: int,
+          slots: int, score: int = SIGMOID, groups: int = 1, top_groups: int = 1, group_best: int = 1, renorm: bool = True,
+          scale: float = 1.0) -> None:
+    """topk for other routers: pick int32 / wts fp32 [rows, slots] from logits [rows, experts] (l_dtype 0 fp16, 1 bf16, 2
+    fp32; rows l_stride apart) by sigmoid or softmax scores, a bias (0: none) for the choice, the top_groups best of `groups`
+    runs of experts (ranked by their one or two best choices), weights renormalised and scaled. Experts with a logit of -inf
+    are never picked; slots that find no expert get -1 and 0."""
+    check(lib().ea_route(stream, logits, l_dtype, l_stride, bias, pick, wts, rows, experts, slots, score, groups, top_groups,
+                         group_best, int(renorm), scale), "route")
 
 
 def swiglu2(stream: int, g: int, u: int, out: int, rows: int, width: int) -> None:

@@ -282,6 +282,82 @@ int ea_swiglu2(ea_stream_t stream, const void* g, const void* u, void* out, uint
  * glue.cu:57). */
 int ea_add_f32(ea_stream_t stream, float* a, const float* b, size_t n);
 
+/* ---- routing in its general form ------------------------------------------------------------------------------ */
+
+#define EA_ROUTE_MAX_EXPERTS 1024
+enum { EA_SCORE_SIGMOID = 0, EA_SCORE_SOFTMAX = 1 };
+/* pick int32 / wts fp32 [rows, slots] from logits [rows, experts] (l_dtype: fp16, bf16 or fp32; rows l_stride elements
+ * apart) for routers that ea_topk8 does not cover. score = sigmoid or softmax of the logits; choice = score + bias (bias fp32
+ * [experts] or NULL). groups > 1: the experts are `groups` equal runs, a run ranks by the sum of its group_best (1 or 2)
+ * largest choices, and the top_groups best runs stay. pick = the `slots` largest choices in order, the lower expert on a tie
+ * (the lower run among runs); wts = score of the pick, divided by (their sum + 1e-20) with renorm, times scale. Scores and
+ * choices are held in 64 bits, so the picks do not depend on how a 32-bit score rounds; wts is rounded once.
+ * An expert whose logit is -inf is out: it is never picked, it gives its run nothing, and where fewer than `slots` are left
+ * the slots behind get pick -1 and weight 0 (a slot without an expert for ea_q4_routed and ea_moe_routed). A NaN choice ranks
+ * below every number, NaNs by the lower expert. 1..EA_ROUTE_MAX_EXPERTS experts, 1..32 slots (EA_TOO_MANY_SLOTS: more, or
+ * more than the kept runs hold), 1..64 groups that divide experts (EA_UNEVEN_SPLIT). No counterpart in the reference, whose
+ * router is ea_topk8's alone. */
+int ea_route(ea_stream_t stream, const void* logits, int l_dtype, uint32_t l_stride, const float* bias, int32_t* pick,
+             float* wts, uint32_t rows, uint32_t experts, uint32_t slots, int score, uint32_t groups, uint32_t top_groups,
+             uint32_t group_best, int renorm, float scale);
+
+/* ---- 4-bit weights in groups ------------------------------------------------------------------------------------ */
+
+/* W[n, k] = scale * q + bias, q in 0..15, one fp16 or bf16 (scale, bias) for each row n and group of 32, 64 or 128
+ * consecutive k: the affine format of the reference's draft model (q4.zig, qmm_group.cu) and of checkpoints that are not
+ * EXL3-encoded. The products take x as it is (fp16 or bf16), multiply by the integers q and apply scale and bias to fp32
+ * sums of a group, so no weight is rounded; a group's bias times its sum of x is added apart, so a row with an infinity
+ * gives infinities or NaN in all of its outputs. */
+#define EA_Q4_MAX_ROWS 65536
+
+/* Bytes of one packed matrix [n, k]; 0 for a group other than 32, 64 or 128, k % group != 0, or n or k 0. */
+size_t ea_q4_bytes(uint32_t n, uint32_t k, uint32_t group);
+/* Lay `count` matrices out for the kernels, once, when a model is loaded: words int32 [count, n, k / 8] (value k of a row in
+ * bits 4 (k % 8) .. + 3 of word k / 8), scales and biases [count, n, k / group] of s_dtype (fp16 or bf16); biases NULL: the
+ * integers stand for q - 8 (bias = -8 scale). out: 16-byte aligned, ea_q4_bytes(n, k, group) a matrix. With words1 .. (gate
+ * and up of experts: both [count, n, k], biases for both or neither) a packed matrix holds both, 8 rows of each in turn:
+ * ea_q4_bytes(16 * ceil(n / 8), k, group) bytes a matrix. */
+int ea_q4_pack(ea_stream_t stream, const void* words0, const void* scales0, const void* biases0, const void* words1,
+               const void* scales1, const void* biases1, void* out, uint32_t n, uint32_t k, uint32_t group, int s_dtype,
+               uint32_t count);
+
+typedef struct ea_q4_linear {
+    uint64_t words;               /* ea_q4_pack's output */
+    uint32_t k, n, group;
+    int32_t s_dtype;
+} ea_q4_linear;
+/* outs[j] [m, n_j] (fp16, bf16 or fp32, contiguous) = x @ W_j^T for 1..3 linears of one k, group and scale type
+ * (EA_NOT_GROUPABLE otherwise), x [m, k] fp16 or bf16 with rows x_stride elements apart (a multiple of 4, x 8-byte aligned:
+ * EA_BAD_ROW_STRIDE / EA_BAD_ARGUMENT), m up to EA_Q4_MAX_ROWS. One launch, no scratch; the outputs may not overlap x. */
+int ea_q4_call(ea_stream_t stream, const ea_q4_linear* const* ls, uint32_t nls, const void* x, int x_dtype,
+               uint32_t x_stride, uint32_t m, const uint64_t* outs, const int* out_dtypes);
+
+/* One layer's routed experts: gate | up packed together ([count] x ea_q4_bytes(16 * ceil(width / 8), dims, group)) and down
+ * ([count] x ea_q4_bytes(dims, width, group)). dims and width are multiples of group; at most 4096 experts. */
+typedef struct ea_q4_experts {
+    uint64_t gu, down;
+    uint32_t count, dims, width, group;
+    int32_t s_dtype;
+    uint32_t reserved;
+} ea_q4_experts;
+/* Scratch for calls of up to `rows` rows with `slots` slots a row, carved from one device buffer (256-byte aligned). It needs
+ * no clearing and may serve layers of no more experts, dims and width in turn; calls that overlap on one scratch race. */
+typedef struct ea_q4_scratch {
+    uint64_t sorted, items, count, h, y;
+    uint32_t rows, slots, experts, dims, width, reserved;
+} ea_q4_scratch;
+size_t ea_q4_scratch_bytes(const ea_q4_experts* ex, uint32_t rows, uint32_t slots);
+int ea_q4_scratch_init(ea_q4_scratch* s, void* base, size_t bytes, const ea_q4_experts* ex, uint32_t rows, uint32_t slots);
+
+/* out [R, dims] (fp16, bf16 or fp32) = sum over the slots of wts * down(silu(gate(x)) * up(x)) of the picked experts: what
+ * ea_moe_routed and ea_prompt_experts_run are for EXL3 experts, for one row to EA_Q4_MAX_ROWS. pick int32 / wts fp32
+ * [R, slots] (slots: the scratch's); a pick outside 0 .. count - 1 is a slot without an expert, a row of such picks gives
+ * zeros, and a row may name an expert twice. The activated values are held as one, two or three bf16 numbers that add up to
+ * them, as many as out's type can show. The same bits on every run. EA_SCRATCH_TOO_SMALL: R above the scratch's rows, or a
+ * layer larger than the one it was made for. */
+int ea_q4_routed(ea_stream_t stream, const void* x, int x_dtype, uint32_t x_stride, const int32_t* pick, const float* wts,
+                 const ea_q4_experts* ex, const ea_q4_scratch* s, void* out, int out_dtype, uint32_t R);
+
 /* ---- the decode layer in one call --------------------------------------------------------------------------- */
 
 /* ffnMain's expert part for a decode window in one call (one launch at one row, five above): pick / wts
