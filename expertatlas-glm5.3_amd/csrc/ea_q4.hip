@@ -1,6 +1,7 @@
 // 4-bit affine weights: the layout's packing and the linears (ea_q4.hpp has the format and the products).
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "ea_host.hpp"
@@ -61,7 +62,7 @@ __global__ void __launch_bounds__(256) q4_pack_kernel(PackSrc s0, PackSrc s1, ui
 struct Q4Job {
     const uint8_t* w;
     void* y;
-    uint32_t n, tile0;  // the job's first tile among all jobs'
+    uint32_t n;
     int y_dtype;
 };
 struct Q4LinArgs {
@@ -73,43 +74,36 @@ struct Q4LinArgs {
     bool sbf;
 };
 
-// A block takes a tile of one job and 16 MT rows; its WK waves take every WK-th chunk and add their sums in wave order.
-template <bool BF, int GPC, int MT, int WK>
+// A block takes NT tiles of one job and 16 MT rows; its WK waves take every WK-th chunk and add their sums in wave order.
+template <bool BF, int GPC, int MT, int NT, int WK, int NB>
 __global__ void __launch_bounds__(64 * WK) q4_linear_kernel(Q4LinArgs a) {
-    __shared__ f4v part[WK][MT][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int ji = 0;
-    while (ji + 1 < a.jobs && blockIdx.x >= a.job[ji + 1].tile0) ++ji;
-    const Q4Job job = a.job[ji];
-    const uint32_t tile = blockIdx.x - job.tile0, m0 = blockIdx.y * 16 * MT;
-    const uint8_t* w = job.w + (size_t)tile * a.chunks * q4_chunk_bytes(GPC);
+    __shared__ f4v part[WK][NT][MT][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Q4Job job = a.job[blockIdx.z];
+    const uint32_t tiles = q4_tiles(job.n), tile0 = blockIdx.x * NT, m0 = blockIdx.y * 16 * MT;
+    if (tile0 >= tiles) return;
+    const size_t tile_bytes = (size_t)a.chunks * q4_chunk_bytes(GPC);
+    const uint32_t first = NT > 1 ? min(tile0, tiles - min(tiles, (uint32_t)NT)) : tile0;  // the last block's tiles overlap
     const uint16_t* row[MT];
-    f4v out[MT];
+    f4v out[NT][MT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
         row[mt] = a.x + (size_t)min(m0 + 16 * mt + (lane & 15), a.m - 1) * a.x_stride;  // rows past m re-read the last
-        out[mt] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
-    }
-    for (uint32_t c = wave; c < a.chunks; c += WK) {
-        const uint8_t* p = w + (size_t)c * q4_chunk_bytes(GPC);
-        const u4v words = reinterpret_cast<const u4v*>(p)[lane];
-        const auto par = q4_params<GPC>(p, lane);
-        u4v x[MT][4];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) q4_rows(row[mt], c, a.k, lane, x[mt]);
-        q4_chunk<BF, GPC, MT>(words, par, x, a.sbf, out);
+        for (int t = 0; t < NT; ++t) out[t][mt] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
     }
+    q4_stream<BF, GPC, MT, NT, NB>(job.w + first * tile_bytes, tiles < NT ? 0 : tile_bytes, wave, WK, a.chunks, row, a.k, lane,
+                                   a.sbf, out);
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) part[wave][mt][lane] = out[mt];
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) part[wave][t][mt][lane] = out[t][mt];
     __syncthreads();
-    const float* all = reinterpret_cast<const float*>(part);
-    for (int i = threadIdx.x; i < 256 * MT; i += 64 * WK) {
-        const int mt = i >> 8, r = (i >> 4) & 15, n = i & 15;
-        const int slot = (mt * 64 + (r >> 2) * 16 + n) * 4 + (r & 3);
-        float v = all[slot];
-        for (int k = 1; k < WK; ++k) v = v + all[k * MT * 256 + slot];
-        const uint32_t mr = m0 + 16 * mt + r, nc = tile * 16 + n;
-        if (mr < a.m && nc < job.n) store_act(job.y, job.y_dtype, (size_t)mr * job.n + nc, v);
+    for (int i = threadIdx.x; i < 256 * MT * NT; i += 64 * WK) {
+        const int n = i & 15, t = (i >> 4) % NT, r = (i / (16 * NT)) & 15, mt = i / (256 * NT);
+        const uint32_t mr = m0 + 16 * mt + r, nc = (first + t) * 16 + n;
+        if (mr < a.m && nc < job.n && (NT == 1 || first + t < tiles))
+            store_act(job.y, job.y_dtype, (size_t)mr * job.n + nc, q4_total<WK, NT, MT>(part, t, mt, r, n));
     }
 }
 
@@ -117,8 +111,11 @@ static int launch_linear(hipStream_t s, const Q4LinArgs& a, uint32_t tiles, bool
     auto go = [&](auto gpc_, auto bf_) {
         constexpr int GPC = decltype(gpc_)::value;
         constexpr bool BF = decltype(bf_)::value;
-        if (a.m <= 16) q4_linear_kernel<BF, GPC, 1, 8><<<dim3(tiles, 1), 512, 0, s>>>(a);
-        else q4_linear_kernel<BF, GPC, 4, 8><<<dim3(tiles, (a.m + 63) / 64), 512, 0, s>>>(a);
+        const unsigned jobs = (unsigned)a.jobs;
+        if (a.m <= 16) {
+            if (tiles * jobs < 512) q4_linear_kernel<BF, GPC, 1, 1, 16, 3><<<dim3(tiles, 1, jobs), 1024, 0, s>>>(a);
+            else q4_linear_kernel<BF, GPC, 1, 2, 8, 3><<<dim3((tiles + 1) / 2, 1, jobs), 512, 0, s>>>(a);
+        } else q4_linear_kernel<BF, GPC, 4, 1, 8, 1><<<dim3(tiles, (a.m + 63) / 64, jobs), 512, 0, s>>>(a);
     };
     auto go_g = [&](auto bf_) {
         if (gpc == 4) go(std::integral_constant<int, 4>{}, bf_);
@@ -180,8 +177,8 @@ int ea_q4_call(ea_stream_t stream, const ea_q4_linear* const* ls, uint32_t nls, 
         if (l->n == 0 || l->k == 0 || (l->s_dtype != F16 && l->s_dtype != BF16)) return EA_BAD_ARGUMENT;
         if (l->k % l->group != 0) return EA_UNEVEN_SPLIT;
         if (l->k != ls[0]->k || l->group != ls[0]->group || l->s_dtype != ls[0]->s_dtype) return EA_NOT_GROUPABLE;
-        a.job[j] = Q4Job{dptr<const uint8_t>(l->words), dptr<void>(outs[j]), l->n, tiles, out_dtypes[j]};
-        tiles += q4_tiles(l->n);
+        a.job[j] = Q4Job{dptr<const uint8_t>(l->words), dptr<void>(outs[j]), l->n, out_dtypes[j]};
+        tiles = std::max(tiles, q4_tiles(l->n));
     }
     if (!x || (x_dtype != F16 && x_dtype != BF16) || (reinterpret_cast<uintptr_t>(x) & 7)) return EA_BAD_ARGUMENT;
     if (x_stride < ls[0]->k || x_stride % 4 != 0) return EA_BAD_ROW_STRIDE;

@@ -70,44 +70,86 @@ __device__ __forceinline__ void q4_scale_bias(uint32_t p, bool bf, float& s, flo
     b = bf ? __builtin_bit_cast(float, p & 0xffff0000u) : h2f((uint16_t)(p >> 16));
 }
 
-// One chunk of one tile against MT groups of 16 rows: out += the chunk's share. a[mt][j]: the rows' A operands of the
-// chunk's four products. The sums of x come from the same operands against ones, which leaves them in the accumulators'
-// own layout. D layout: lane l holds row 4 (l >> 4) + i, weight row l & 15.
-template <bool BF, int GPC, int MT>
-__device__ __forceinline__ void q4_chunk(const u4v& words, const Q4Params<GPC>& par, const u4v (&a)[MT][4], bool sbf,
-                                         f4v (&out)[MT]) {
+// A chunk of NT tiles against MT groups of 16 rows: out += the chunk's share. a[mt][j]: the rows' A operands of the chunk's
+// four products. The sums of x come from the same operands against ones, which leaves them in the accumulators' own layout
+// (lane l: rows 4 (l >> 4) + i, weight row l & 15).
+template <bool BF, int GPC, int MT, int NT>
+__device__ __forceinline__ void q4_chunk(const u4v (&words)[NT], const Q4Params<GPC> (&par)[NT], const u4v (&a)[MT][4],
+                                         bool sbf, f4v (&out)[NT][MT]) {
     constexpr int JPG = 4 / GPC;
+    const f4v zero{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int g = 0; g < GPC; ++g) {
-        f4v acc[MT], xs[MT];
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) acc[mt] = xs[mt] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int j = 0; j < JPG; ++j) {
-            const u4v b = q4_values<BF>(words[g * JPG + j]);
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                acc[mt] = q4_mfma<BF>(a[mt][g * JPG + j], b, acc[mt]);
-                xs[mt] = q4_mfma<BF>(a[mt][g * JPG + j], q4_ones<BF>(), xs[mt]);
-            }
-        }
-        float s, b;
-        q4_scale_bias(par.w[g], sbf, s, b);
+        f4v xs[MT];
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                out[mt][i] = __builtin_fmaf(b, xs[mt][i], __builtin_fmaf(s, acc[mt][i], out[mt][i]));
+            for (int j = 0; j < JPG; ++j) xs[mt] = q4_mfma<BF>(a[mt][g * JPG + j], q4_ones<BF>(), j ? xs[mt] : zero);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            f4v acc[MT];
+#pragma unroll
+            for (int j = 0; j < JPG; ++j) {
+                const u4v b = q4_values<BF>(words[t][g * JPG + j]);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) acc[mt] = q4_mfma<BF>(a[mt][g * JPG + j], b, j ? acc[mt] : zero);
+            }
+            float s, b;
+            q4_scale_bias(par[t].w[g], sbf, s, b);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    out[t][mt][i] = __builtin_fmaf(b, xs[mt][i], __builtin_fmaf(s, acc[mt][i], out[t][mt][i]));
+        }
     }
 }
 
-// The lane's A operands of one chunk of a row of 16-bit activations; zeros from k on (k a multiple of 32).
+// The lane's A operands of one chunk of a row of 16-bit activations (k a multiple of 32). Past k, where the weights, scales
+// and biases are zeros, values of the row before it stand in: times zero they add nothing, as long as the row is finite.
 __device__ __forceinline__ void q4_rows(const uint16_t* row, uint32_t chunk, uint32_t k, int lane, u4v (&a)[4]) {
     const uint16_t* p = row + (size_t)chunk * Q4_CHUNK + 8 * (lane >> 4);
-    const int left = (int)(k - chunk * Q4_CHUNK);
+    const int last = (int)(k - chunk * Q4_CHUNK) - 32;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-        a[j] = 32 * j < left ? (u4v) * reinterpret_cast<const u4v_a8*>(p + 32 * j) : u4v{0, 0, 0, 0};
+    for (int j = 0; j < 4; ++j) a[j] = (u4v) * reinterpret_cast<const u4v_a8*>(p + min(32 * j, last));
+}
+
+// The tiles at w, w + tile_bytes, .. against MT groups of 16 rows over the chunks c0, c0 + step, ..: the loads of NB chunks
+// are issued before the first of their products.
+template <bool BF, int GPC, int MT, int NT, int NB>
+__device__ __forceinline__ void q4_stream(const uint8_t* w, size_t tile_bytes, uint32_t c0, uint32_t step, uint32_t chunks,
+                                          const uint16_t* const (&row)[MT], uint32_t k, int lane, bool sbf,
+                                          f4v (&out)[NT][MT]) {
+    for (uint32_t c = c0; c < chunks; c += step * NB) {
+        u4v words[NB][NT], x[NB][MT][4];
+        Q4Params<GPC> par[NB][NT];
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            const uint32_t ci = min(c + step * i, chunks - 1);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const uint8_t* p = w + t * tile_bytes + (size_t)ci * q4_chunk_bytes(GPC);
+                words[i][t] = reinterpret_cast<const u4v*>(p)[lane];
+                par[i][t] = q4_params<GPC>(p, lane);
+            }
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) q4_rows(row[mt], ci, k, lane, x[i][mt]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+            if (c + step * i < chunks) q4_chunk<BF, GPC, MT, NT>(words[i], par[i], x[i], sbf, out);
+    }
+}
+
+// Value (row r of group mt, weight row n of tile t) summed over the waves' parts, in wave order.
+template <int WK, int NT, int MT>
+__device__ __forceinline__ float q4_total(const f4v (&part)[WK][NT][MT][64], int t, int mt, int r, int n) {
+    const float* all = reinterpret_cast<const float*>(part) + ((t * MT + mt) * 64 + (r >> 2) * 16 + n) * 4 + (r & 3);
+    float v = all[0];
+#pragma unroll
+    for (int k = 1; k < WK; ++k) v = v + all[k * NT * MT * 256];
+    return v;
 }
 
 }  // namespace ea
