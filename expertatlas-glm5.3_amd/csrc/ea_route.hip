@@ -2,8 +2,7 @@
 // groups of experts of which the best are kept, the k largest choices, weights that are renormalised and scaled.
 //
 // A choice is compared in 64 bits: the picks are whole numbers, two choices can lie closer than a 32-bit sigmoid's error, and
-// a balance bias moves them to within it on purpose, so that the picks would otherwise depend on how a sigmoid rounds. A
-// wave takes a row, lane l its experts l, l + 64, ..
+// a balance bias moves them to within it on purpose, so that the picks would otherwise depend on how a sigmoid rounds.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -36,141 +35,175 @@ __device__ __forceinline__ double choice_of(uint64_t k) {
     return __builtin_bit_cast(double, (k >> 63) ? k & ~(1ull << 63) : k == 1 ? 0x7ff8000000000000ull : ~k);
 }
 
-template <int M, typename T>
-__device__ __forceinline__ T lane_xor64(T v) {
-    const uint64_t u = __builtin_bit_cast(uint64_t, v);
-    const float lo = lane_xor<M>(__builtin_bit_cast(float, (uint32_t)u));
-    const float hi = lane_xor<M>(__builtin_bit_cast(float, (uint32_t)(u >> 32)));
-    return __builtin_bit_cast(T, (uint64_t)__builtin_bit_cast(uint32_t, lo) | (uint64_t)__builtin_bit_cast(uint32_t, hi) << 32);
+template <int CTL>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTL, 0xf, 0xf, true);
 }
-
-// f over the wave by the butterfly: every lane ends with the same value.
-template <typename T, typename F>
-__device__ __forceinline__ T wave_all(T v, F f) {
-    v = f(v, lane_xor64<32>(v));
-    v = f(v, lane_xor64<16>(v));
-    v = f(v, lane_xor64<8>(v));
-    v = f(v, lane_xor64<4>(v));
-    v = f(v, lane_xor64<2>(v));
-    return f(v, lane_xor64<1>(v));
+// f over the L = 16 or 64 lanes of a row: every lane ends with the result (f commutative and associative).
+template <int L, typename F>
+__device__ __forceinline__ uint32_t row_all(uint32_t v, F f) {
+    v = f(v, dpp<0xB1>(v));   // quad_perm 1,0,3,2
+    v = f(v, dpp<0x4E>(v));   // quad_perm 2,3,0,1
+    v = f(v, dpp<0x141>(v));  // row_half_mirror
+    v = f(v, dpp<0x140>(v));  // row_mirror
+    if constexpr (L == 64) {
+        const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        v = f((uint32_t)a[0], (uint32_t)a[1]);
+        const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        v = f((uint32_t)b[0], (uint32_t)b[1]);
+    }
+    return v;
 }
-
-__device__ __forceinline__ double read_lane(double v, int lane) {
-    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+template <int L>
+__device__ __forceinline__ uint32_t row_max(uint32_t v) {
+    return row_all<L>(v, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+}
+template <int L>
+__device__ __forceinline__ double row_sum(double v) {
+#pragma unroll
+    for (int m = 1; m < L; m <<= 1) v = v + __shfl_xor(v, m, 64);
+    return v;
+}
+__device__ __forceinline__ uint64_t read_lane(uint64_t u, int lane) {
     const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)u, lane), hi = __builtin_amdgcn_readlane((uint32_t)(u >> 32), lane);
-    return __builtin_bit_cast(double, (uint64_t)lo | (uint64_t)hi << 32);
+    return (uint64_t)lo | (uint64_t)hi << 32;
+}
+// What one lane of a wave wrote to LDS before is there for the others: LDS works in order, the compiler has to as well.
+__device__ __forceinline__ void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
 }
 
-constexpr int ROUTE_WAVES = 4;
+__device__ __forceinline__ float load_logit(const RouteArgs& a, size_t i) { return load_act(a.logits, a.dtype, i); }
 
-template <int EPL, bool GROUPS>
-__global__ void __launch_bounds__(64 * ROUTE_WAVES) route_kernel(RouteArgs a) {
-    __shared__ uint64_t keys[GROUPS ? ROUTE_WAVES : 1][GROUPS ? 64 * EPL : 1];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint32_t row = blockIdx.x * ROUTE_WAVES + wave;
-    if (row >= a.rows) return;  // no barrier below: a wave works alone
-    float x[EPL];
-    double s[EPL];
+// L lanes take a row, lane l its experts l, l + L, .. (EPL of them); a wave has 64 / L rows. The work is instructions, not
+// bytes (a 64-bit sigmoid of each logit, then the slots in turn: a row's largest key, found by its upper half first, which
+// only ties to 20 bits follow with the lower half and the expert's number). So many rows take 16 lanes each, which shares the
+// steps over the lanes between four rows; few take a wave each, for the shorter chain.
+template <int EPL, int L, bool GROUPS>
+__global__ void __launch_bounds__(256) route_kernel(RouteArgs a) {
+    constexpr int ROWS = 256 / L;
+    __shared__ double score[ROWS][EPL * L];
+    __shared__ int32_t got[ROWS][32];
+    __shared__ uint64_t keys[GROUPS ? ROWS : 1][GROUPS ? EPL * L : 1];
+    const int lane = threadIdx.x & 63, l = threadIdx.x % L, w = threadIdx.x / L;
+    if (blockIdx.x * (uint32_t)ROWS + (threadIdx.x & ~63u) / L >= a.rows) return;  // a whole wave; no barrier below
+    const uint32_t row = min(blockIdx.x * (uint32_t)ROWS + w, a.rows - 1);  // lanes past the last row repeat it
+    float x[EPL], bias[EPL];
     uint64_t key[EPL];
 #pragma unroll
     for (int j = 0; j < EPL; ++j) {
-        const int e = lane + 64 * j;
-        x[j] = e < a.experts ? load_act(a.logits, a.dtype, (size_t)row * a.stride + e) : -__builtin_inff();
+        const int e = l + L * j;
+        x[j] = e < a.experts ? load_logit(a, (size_t)row * a.stride + e) : -__builtin_inff();
+        bias[j] = a.bias && e < a.experts ? a.bias[e] : 0.0f;
+    }
+    got[w][l % 32] = -1;
+    if (L < 32) got[w][l + L] = -1;
+    double m = 0.0, part = 0.0;
+    if (a.softmax) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) top = max(top, order_key(x[j]));
+        top = row_max<L>(top);  // of the numbers: a NaN makes the sum NaN by itself
+        const float t = __builtin_bit_cast(float, (top & 0x80000000u) ? top & 0x7fffffffu : ~top);
+        m = top <= 1 || t == -__builtin_inff() ? 0.0 : (double)t;
+    }
+    double s[EPL];
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) {
+        s[j] = a.softmax ? exp((double)x[j] - m) : 1.0 / (1.0 + exp(-(double)x[j]));
+        part += s[j];
     }
     if (a.softmax) {
-        float top = x[0];
-#pragma unroll
-        for (int j = 1; j < EPL; ++j) top = __builtin_fmaxf(top, x[j]);
-        const double m = wave_all((double)top, [](double p, double q) { return __builtin_fmax(p, q); });
-        const double m0 = m == -__builtin_inf() ? 0.0 : m;
-        double sum = 0.0;
-#pragma unroll
-        for (int j = 0; j < EPL; ++j) {
-            s[j] = exp((double)x[j] - m0);
-            sum += s[j];
-        }
-        sum = wave_all(sum, [](double p, double q) { return p + q; });
+        const double sum = row_sum<L>(part);
 #pragma unroll
         for (int j = 0; j < EPL; ++j) s[j] = s[j] / sum;
-    } else {
-#pragma unroll
-        for (int j = 0; j < EPL; ++j) s[j] = 1.0 / (1.0 + exp(-(double)x[j]));
     }
 #pragma unroll
     for (int j = 0; j < EPL; ++j) {
-        const int e = lane + 64 * j;
-        const double c = a.bias && e < a.experts ? s[j] + (double)a.bias[e] : s[j];
-        key[j] = x[j] == -__builtin_inff() ? 0ull : choice_key(c);
+        score[w][l + L * j] = s[j];
+        key[j] = x[j] == -__builtin_inff() ? 0ull : choice_key(a.bias ? s[j] + (double)bias[j] : s[j]);
     }
     if constexpr (GROUPS) {
+        static_assert(L == 64, "a group's lanes are read across the wave");
         const int size = a.experts / a.groups;
 #pragma unroll
-        for (int j = 0; j < EPL; ++j) keys[wave][lane + 64 * j] = key[j];
-        __builtin_amdgcn_wave_barrier();
-        // lane g ranks group g by the sum of its one or two best choices (those that it has)
+        for (int j = 0; j < EPL; ++j) keys[w][l + L * j] = key[j];
+        wave_fence();
+        // per neighbouring lanes (a power of two) rank a group by the sum of its one or two best choices, those it has
+        const int per = 1 << (31 - __builtin_clz(64 / a.groups)), g = lane / per;
         uint64_t first = 0, second = 0;
-        if (lane < a.groups)
-            for (int i = 0; i < size; ++i) {
-                const uint64_t k = keys[wave][lane * size + i];
-                second = k > first ? first : k > second ? k : second;
-                first = k > first ? k : first;
-            }
+        for (int i = lane % per; g < a.groups && i < size; i += per) {
+            const uint64_t k = keys[w][g * size + i];
+            second = k > first ? first : k > second ? k : second;
+            first = k > first ? k : first;
+        }
+        for (int d = 1; d < per; d <<= 1) {
+            const uint64_t of = __shfl_xor(first, d, 64), os = __shfl_xor(second, d, 64), s2 = os > second ? os : second;
+            const uint64_t lo = of > first ? first : of;
+            second = lo > s2 ? lo : s2;
+            first = of > first ? of : first;
+        }
         uint64_t rank = first;
         if (a.group_best == 2 && second) rank = choice_key(choice_of(first) + choice_of(second));
         int before = 0;
-        for (int g = 0; g < a.groups; ++g) {
-            const uint64_t o = __builtin_bit_cast(uint64_t, read_lane(__builtin_bit_cast(double, rank), g));
-            before += o > rank || (o == rank && g < lane);
+        for (int o = 0; o < a.groups; ++o) {
+            const uint64_t r = read_lane(rank, o * per);
+            before += r > rank || (r == rank && o < g);
         }
-        const uint64_t kept = __ballot(lane < a.groups && before < a.top_groups);
+        const uint64_t kept = __ballot(g < a.groups && before < a.top_groups);  // bit per * g
 #pragma unroll
         for (int j = 0; j < EPL; ++j) {
-            const int e = lane + 64 * j;
-            if (e < a.experts && !(kept >> (e / size) & 1)) key[j] = 0;
+            const int e = l + L * j;
+            if (e < a.experts && !(kept >> (e / size * per) & 1)) key[j] = 0;
         }
     }
-    // the slots in turn: the largest key of the wave, the lowest expert that holds it
-    double sum = 0.0, mine = 0.0;
-    int mine_e = -1;
+    wave_fence();
+    // the slots in turn
+    const auto row_bits = [&](uint64_t b) { return L == 64 ? b : b >> (lane & ~(L - 1)) & 0xffffull; };
     for (int k = 0; k < a.slots; ++k) {
         uint64_t best = key[0];
+        int at = l;
 #pragma unroll
-        for (int j = 1; j < EPL; ++j) best = key[j] > best ? key[j] : best;
-        best = wave_all(best, [](uint64_t p, uint64_t q) { return p > q ? p : q; });
-        if (best == 0) break;  // none left: this slot and the ones after it stay empty
-        int at = -1, who = 0;
-        double w = 0.0;
-#pragma unroll
-        for (int j = EPL - 1; j >= 0; --j) {
-            const uint64_t has = __ballot(key[j] == best);
-            if (has) {
-                who = __builtin_ctzll(has);
-                at = who + 64 * j;
-                w = read_lane(s[j], who);
-            }
+        for (int j = 1; j < EPL; ++j) {
+            const bool more = key[j] > best;
+            best = more ? key[j] : best;
+            at = more ? l + L * j : at;
         }
-#pragma unroll
-        for (int j = 0; j < EPL; ++j) key[j] = at == lane + 64 * j ? 0 : key[j];
-        sum += w;
-        if (lane == k) {
-            mine = w;
-            mine_e = at;
+        const uint32_t hi = (uint32_t)(best >> 32), top = row_max<L>(hi);
+        bool win = hi == top && best != 0;
+        const uint64_t tied = row_bits(__ballot(win));
+        if (__ballot((tied & (tied - 1)) != 0)) {  // equal upper halves in some row
+            const uint32_t lo = win ? (uint32_t)best : 0, ltop = row_max<L>(lo);
+            win = win && lo == ltop;
+            const uint32_t last = row_max<L>(win ? 0xffffffffu - at : 0);
+            win = win && 0xffffffffu - at == last;
         }
+        if (win) got[w][k] = at;
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) key[j] = win && at == l + L * j ? 0 : key[j];
     }
-    if (lane < a.slots) {
-        const size_t o = (size_t)row * a.slots + lane;
-        const double w = mine_e < 0 ? 0.0 : a.renorm ? mine / (sum + 1e-20) : mine;
-        a.pick[o] = mine_e;
-        a.wts[o] = (float)(w * (double)a.scale);
+    wave_fence();
+    double sum = 0.0;
+    if (a.renorm) {
+        for (int k = l; k < a.slots; k += L) sum += got[w][k] < 0 ? 0.0 : score[w][got[w][k]];
+        sum = row_sum<L>(sum) + 1e-20;
+    }
+    if (blockIdx.x * (uint32_t)ROWS + w >= a.rows) return;
+    for (int k = l; k < a.slots; k += L) {
+        const int e = got[w][k];
+        const double v = e < 0 ? 0.0 : a.renorm ? score[w][e] / sum : score[w][e];
+        a.pick[(size_t)row * a.slots + k] = e;
+        a.wts[(size_t)row * a.slots + k] = (float)(v * (double)a.scale);
     }
 }
 
 static int launch_route(hipStream_t s, const RouteArgs& a) {
-    const unsigned blocks = (a.rows + ROUTE_WAVES - 1) / ROUTE_WAVES;
     auto go = [&](auto epl) {
         constexpr int EPL = decltype(epl)::value;
-        if (a.groups > 1) route_kernel<EPL, true><<<blocks, 64 * ROUTE_WAVES, 0, s>>>(a);
-        else route_kernel<EPL, false><<<blocks, 64 * ROUTE_WAVES, 0, s>>>(a);
+        if (a.groups > 1) route_kernel<EPL, 64, true><<<(a.rows + 3) / 4, 256, 0, s>>>(a);
+        else if (EPL > 4 || a.rows < 1024) route_kernel<EPL, 64, false><<<(a.rows + 3) / 4, 256, 0, s>>>(a);
+        else route_kernel<4 * std::min(EPL, 4), 16, false><<<(a.rows + 15) / 16, 256, 0, s>>>(a);
     };
     if (a.experts <= 64) go(std::integral_constant<int, 1>{});
     else if (a.experts <= 128) go(std::integral_constant<int, 2>{});
