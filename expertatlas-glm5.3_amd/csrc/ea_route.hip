@@ -39,16 +39,18 @@ template <int CTL>
 __device__ __forceinline__ uint32_t dpp(uint32_t v) {
     return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTL, 0xf, 0xf, true);
 }
-// f over the L = 16 or 64 lanes of a row: every lane ends with the result (f commutative and associative).
+// f over the L = 16, 32 or 64 lanes of a row: every lane ends with the result (f commutative and associative).
 template <int L, typename F>
 __device__ __forceinline__ uint32_t row_all(uint32_t v, F f) {
     v = f(v, dpp<0xB1>(v));   // quad_perm 1,0,3,2
     v = f(v, dpp<0x4E>(v));   // quad_perm 2,3,0,1
     v = f(v, dpp<0x141>(v));  // row_half_mirror
     v = f(v, dpp<0x140>(v));  // row_mirror
-    if constexpr (L == 64) {
+    if constexpr (L >= 32) {
         const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
         v = f((uint32_t)a[0], (uint32_t)a[1]);
+    }
+    if constexpr (L == 64) {
         const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
         v = f((uint32_t)b[0], (uint32_t)b[1]);
     }
@@ -74,12 +76,22 @@ __device__ __forceinline__ void wave_fence() {
     __builtin_amdgcn_wave_barrier();
 }
 
-__device__ __forceinline__ float load_logit(const RouteArgs& a, size_t i) { return load_act(a.logits, a.dtype, i); }
+// 1 / (1 + exp(-x)) in 64 bits: v_rcp_f64's estimate and two Newton steps (an IEEE division takes twice the instructions).
+__device__ __forceinline__ double sigmoid64(double x) {
+    const double d = 1.0 + exp(__builtin_fmin(-x, 709.0));
+    double r = __builtin_amdgcn_rcp(d);
+    r = __builtin_fma(r, __builtin_fma(-d, r, 1.0), r);
+    r = __builtin_fma(r, __builtin_fma(-d, r, 1.0), r);
+    return x != x ? x : r;
+}
 
-// L lanes take a row, lane l its experts l, l + L, .. (EPL of them); a wave has 64 / L rows. The work is instructions, not
-// bytes (a 64-bit sigmoid of each logit, then the slots in turn: a row's largest key, found by its upper half first, which
-// only ties to 20 bits follow with the lower half and the expert's number). So many rows take 16 lanes each, which shares the
-// steps over the lanes between four rows; few take a wave each, for the shorter chain.
+// L lanes take a row, lane l its experts l, l + L, .. (EPL of them); a wave has 64 / L rows. What bounds it are instructions
+// and their latencies, not bytes (256 experts x 4096 rows are 4.5 MB, 0.9 us): a 64-bit sigmoid of each logit, then the slots
+// in turn, a row's largest key found by its upper half first, which only ties to 20 bits follow with the lower half and the
+// expert's number. A wave a row has the shortest chain; 32 lanes a row share the steps over the lanes between two rows, which
+// pays when every SIMD has several waves anyway. 256 experts, 8 slots, kernel times, 64 and 32 lanes: 1 row 4.6 us, 512 rows
+// 5.3 and 6.7, 2048 rows 6.2 and 6.8, 4096 rows 8.4 and 7.8 (16 lanes: 9.8 at any of these). The loads of a row had been
+// behind conditions, waited for one by one: 1 row 5.6 us, 4096 rows 12.3 then.
 template <int EPL, int L, bool GROUPS>
 __global__ void __launch_bounds__(256) route_kernel(RouteArgs a) {
     constexpr int ROWS = 256 / L;
@@ -91,11 +103,27 @@ __global__ void __launch_bounds__(256) route_kernel(RouteArgs a) {
     const uint32_t row = min(blockIdx.x * (uint32_t)ROWS + w, a.rows - 1);  // lanes past the last row repeat it
     float x[EPL], bias[EPL];
     uint64_t key[EPL];
+    {  // every load before the first use (experts past the last re-read it)
+        const size_t at = (size_t)row * a.stride;
+        if (a.dtype == F32) {
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) {
-        const int e = l + L * j;
-        x[j] = e < a.experts ? load_logit(a, (size_t)row * a.stride + e) : -__builtin_inff();
-        bias[j] = a.bias && e < a.experts ? a.bias[e] : 0.0f;
+            for (int j = 0; j < EPL; ++j) x[j] = static_cast<const float*>(a.logits)[at + min(l + L * j, a.experts - 1)];
+        } else {
+            uint16_t h[EPL];
+#pragma unroll
+            for (int j = 0; j < EPL; ++j) h[j] = static_cast<const uint16_t*>(a.logits)[at + min(l + L * j, a.experts - 1)];
+#pragma unroll
+            for (int j = 0; j < EPL; ++j) x[j] = a.dtype == BF16 ? bf2f(h[j]) : h2f(h[j]);
+        }
+        if (a.bias) {
+#pragma unroll
+            for (int j = 0; j < EPL; ++j) bias[j] = a.bias[min(l + L * j, a.experts - 1)];
+        } else {
+#pragma unroll
+            for (int j = 0; j < EPL; ++j) bias[j] = 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) x[j] = l + L * j < a.experts ? x[j] : -__builtin_inff();
     }
     got[w][l % 32] = -1;
     if (L < 32) got[w][l + L] = -1;
@@ -109,15 +137,18 @@ __global__ void __launch_bounds__(256) route_kernel(RouteArgs a) {
         m = top <= 1 || t == -__builtin_inff() ? 0.0 : (double)t;
     }
     double s[EPL];
-#pragma unroll
-    for (int j = 0; j < EPL; ++j) {
-        s[j] = a.softmax ? exp((double)x[j] - m) : 1.0 / (1.0 + exp(-(double)x[j]));
-        part += s[j];
-    }
     if (a.softmax) {
-        const double sum = row_sum<L>(part);
 #pragma unroll
-        for (int j = 0; j < EPL; ++j) s[j] = s[j] / sum;
+        for (int j = 0; j < EPL; ++j) {
+            s[j] = exp((double)x[j] - m);
+            part += s[j];
+        }
+        const double r = 1.0 / row_sum<L>(part);
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) s[j] = s[j] * r;
+    } else {
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) s[j] = sigmoid64((double)x[j]);
     }
 #pragma unroll
     for (int j = 0; j < EPL; ++j) {
@@ -160,7 +191,7 @@ __global__ void __launch_bounds__(256) route_kernel(RouteArgs a) {
     }
     wave_fence();
     // the slots in turn
-    const auto row_bits = [&](uint64_t b) { return L == 64 ? b : b >> (lane & ~(L - 1)) & 0xffffull; };
+    const auto row_bits = [&](uint64_t b) { return L == 64 ? b : b >> (lane & ~(L - 1)) & ((1ull << (L & 63)) - 1); };
     for (int k = 0; k < a.slots; ++k) {
         uint64_t best = key[0];
         int at = l;
@@ -202,8 +233,8 @@ static int launch_route(hipStream_t s, const RouteArgs& a) {
     auto go = [&](auto epl) {
         constexpr int EPL = decltype(epl)::value;
         if (a.groups > 1) route_kernel<EPL, 64, true><<<(a.rows + 3) / 4, 256, 0, s>>>(a);
-        else if (EPL > 4 || a.rows < 1024) route_kernel<EPL, 64, false><<<(a.rows + 3) / 4, 256, 0, s>>>(a);
-        else route_kernel<4 * std::min(EPL, 4), 16, false><<<(a.rows + 15) / 16, 256, 0, s>>>(a);
+        else if (EPL > 4 || a.rows < 4096) route_kernel<EPL, 64, false><<<(a.rows + 3) / 4, 256, 0, s>>>(a);
+        else route_kernel<2 * std::min(EPL, 4), 32, false><<<(a.rows + 7) / 8, 256, 0, s>>>(a);
     };
     if (a.experts <= 64) go(std::integral_constant<int, 1>{});
     else if (a.experts <= 128) go(std::integral_constant<int, 2>{});
