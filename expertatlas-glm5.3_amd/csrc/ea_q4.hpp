@@ -115,8 +115,8 @@ __device__ __forceinline__ void q4_rows(const uint16_t* row, uint32_t chunk, uin
 }
 
 // The tiles at w, w + tile_bytes, .. against MT groups of 16 rows over the chunks c0, c0 + step, ..: the loads of NB chunks
-// are issued before the first of their products.
-template <bool BF, int GPC, int MT, int NT, int NB>
+// are issued before the first of their products. With SOME, a lane whose row is null reads nothing and multiplies zeros.
+template <bool BF, int GPC, int MT, int NT, int NB, bool SOME = false>
 __device__ __forceinline__ void q4_stream(const uint8_t* w, size_t tile_bytes, uint32_t c0, uint32_t step, uint32_t chunks,
                                           const uint16_t* const (&row)[MT], uint32_t k, int lane, bool sbf,
                                           f4v (&out)[NT][MT]) {
@@ -132,8 +132,20 @@ __device__ __forceinline__ void q4_stream(const uint8_t* w, size_t tile_bytes, u
                 words[i][t] = reinterpret_cast<const u4v*>(p)[lane];
                 par[i][t] = q4_params<GPC>(p, lane);
             }
+            if constexpr (!SOME)
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) q4_rows(row[mt], ci, k, lane, x[i][mt]);
+                for (int mt = 0; mt < MT; ++mt) q4_rows(row[mt], ci, k, lane, x[i][mt]);
+        }
+        if constexpr (SOME) {
+            static_assert(MT == 1, "one row a lane");
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[i][0][j] = u4v{0, 0, 0, 0};
+            if (row[0]) {
+#pragma unroll
+                for (int i = 0; i < NB; ++i) q4_rows(row[0], min(c + step * i, chunks - 1), k, lane, x[i][0]);
+            }
         }
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll

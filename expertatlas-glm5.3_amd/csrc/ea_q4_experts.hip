@@ -1,11 +1,12 @@
 // Routed experts with 4-bit weights in groups: out[r] = sum over slots of wts * down_e(silu(gate_e x) * (up_e x)).
 //
-// The rows' picks are sorted by expert and cut into items (an expert and up to 16 Q4_MT of its pairs); a block multiplies
-// an item's rows by one tile of the expert's gate|up (8 columns of each) and writes the activated pairs; another multiplies
-// those by one tile of the down projection; the last launch adds a row's slots in order. A pair's values depend neither on
-// the others of its item nor on their order, so the results are the same on every run.
+// The rows' picks are sorted by expert and cut into items (an expert and up to 16 of its pairs); a block multiplies an
+// item's rows by tiles of the expert's gate|up (8 columns of each) and writes the activated pairs; another multiplies those
+// by tiles of the down projection; the last launch adds a row's slots in order. A pair's values depend neither on the others
+// of its item nor on their order, so the results are the same on every run.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "ea_host.hpp"
@@ -13,8 +14,9 @@
 
 namespace ea {
 
-constexpr int Q4_MT = 4;
 constexpr uint32_t Q4_MAX_EXPERTS = 4096;
+constexpr uint32_t Q4_ITEM = 16;                       // rows an item
+constexpr uint32_t Q4_ROWS = 16, Q4_PAIRS = Q4_ROWS * 32;  // rows and pairs that are grouped beside the first products
 
 struct Q4Item {
     int32_t expert, first, count, pad;
@@ -27,10 +29,10 @@ struct Q4MoeArgs {
     const float* wts;
     const uint8_t *gu, *down;
     size_t gu_bytes, down_bytes;  // one expert's
-    int32_t *sorted, *nitems;
-    Q4Item* items;
-    uint16_t* h;  // bf16 [terms][pairs][width]
-    float* y;     // fp32 [pairs][dims]
+    int32_t *sorted, *nitems;     // pairs by expert; the number of items
+    Q4Item* items;                // runs of sorted
+    uint16_t* h;                  // bf16 [terms][pairs][width]
+    float* y;                     // fp32 [pairs][dims]
     void* out;
     uint32_t rows, pairs, dims, width, experts, slots;
     int out_dtype;
@@ -53,7 +55,7 @@ __global__ void __launch_bounds__(1024) q4_group_kernel(Q4MoeArgs a) {
     // exclusive scans of the counts and the item counts, 1024 experts a step
     uint32_t base = 0, ibase = 0;
     for (uint32_t e0 = 0; e0 < a.experts; e0 += 1024) {
-        const uint32_t e = e0 + t, c = e < a.experts ? count[e] : 0, n = (c + 16 * Q4_MT - 1) / (16 * Q4_MT);
+        const uint32_t e = e0 + t, c = e < a.experts ? count[e] : 0, n = (c + Q4_ITEM - 1) / Q4_ITEM;
         uint32_t v = c, w = n;
         for (int d = 1; d < 64; d <<= 1) {
             const uint32_t pv = __shfl_up(v, d), pw = __shfl_up(w, d);
@@ -71,8 +73,7 @@ __global__ void __launch_bounds__(1024) q4_group_kernel(Q4MoeArgs a) {
         const uint32_t first = bv + v - c, item = bw + w - n;
         if (e < a.experts) start[e] = first;
         for (uint32_t i = 0; i < n; ++i)
-            a.items[item + i] = Q4Item{(int32_t)e, (int32_t)(first + i * 16 * Q4_MT),
-                                       (int32_t)min(c - i * 16 * Q4_MT, 16u * Q4_MT), 0};
+            a.items[item + i] = Q4Item{(int32_t)e, (int32_t)(first + i * Q4_ITEM), (int32_t)min(c - i * Q4_ITEM, Q4_ITEM), 0};
         __syncthreads();
     }
     if (t == 0) *a.nitems = (int32_t)ibase;
@@ -80,6 +81,66 @@ __global__ void __launch_bounds__(1024) q4_group_kernel(Q4MoeArgs a) {
         const uint32_t e = (uint32_t)a.pick[p];
         if (e < a.experts) a.sorted[atomicAdd(&start[e], 1u)] = (int32_t)p;
     }
+}
+
+// The same for up to 16 rows, in the order of the experts' first pairs, by a block beside the first products (picks: the
+// call's, in LDS, changed). An expert is one item, and a row that names it again is left out: the last launch gives its
+// weight to the first naming.
+template <int THREADS>
+__device__ void q4_group_rows(const Q4MoeArgs& a, int32_t* picks) {
+    __shared__ int16_t owner[Q4_PAIRS], before[Q4_PAIRS], count[Q4_PAIRS], first[Q4_PAIRS];
+    int32_t once[(Q4_PAIRS + THREADS - 1) / THREADS];
+    for (uint32_t p = threadIdx.x, i = 0; p < a.pairs; p += THREADS, ++i) {
+        int32_t e = picks[p];
+        e = (uint32_t)e < a.experts ? e : -1;
+        for (uint32_t q = p - p % a.slots; q < p; ++q) e = picks[q] == e ? -1 : e;
+        once[i] = e;
+        count[p] = 0;
+    }
+    __syncthreads();
+    for (uint32_t p = threadIdx.x, i = 0; p < a.pairs; p += THREADS, ++i) picks[p] = once[i];
+    __syncthreads();
+    for (uint32_t p = threadIdx.x; p < a.pairs; p += THREADS) {
+        const int32_t e = picks[p];
+        uint32_t n = 0, own = p, all = 0;
+        if (e >= 0) {
+#pragma unroll 4
+            for (uint32_t q = 0; q < a.pairs; ++q) {
+                const bool same = picks[q] == e;
+                own = same && all == 0 ? q : own;
+                n += same && q < p;
+                all += same;
+            }
+        }
+        owner[p] = (int16_t)own;
+        before[p] = e >= 0 ? (int16_t)n : -1;
+        count[p] = (int16_t)all;
+    }
+    __syncthreads();
+    if (threadIdx.x < 64) {
+        int items = 0, at = 0;
+        for (uint32_t p0 = 0; p0 < a.pairs; p0 += 64) {
+            const uint32_t p = p0 + threadIdx.x;
+            const bool fresh = p < a.pairs && before[p] == 0;
+            const int c = fresh ? count[p] : 0;
+            int sum = c;
+            for (int d = 1; d < 64; d <<= 1) {
+                const int o = __shfl_up(sum, d);
+                sum += (int)threadIdx.x >= d ? o : 0;
+            }
+            const uint64_t all = __ballot(fresh);
+            if (fresh) {
+                first[p] = (int16_t)(at + sum - c);
+                a.items[items + __builtin_popcountll(all & ((1ull << threadIdx.x) - 1))] = Q4Item{picks[p], at + sum - c, c, 0};
+            }
+            items += __builtin_popcountll(all);
+            at += __shfl(sum, 63);
+        }
+        if (threadIdx.x == 0) *a.nitems = items;
+    }
+    __syncthreads();
+    for (uint32_t p = threadIdx.x; p < a.pairs; p += THREADS)
+        if (before[p] >= 0) a.sorted[first[owner[p]] + before[p]] = (int32_t)p;
 }
 
 __device__ __forceinline__ float swiglu(float g, float u) { return g / (1.0f + expf_path(0.0f - g)) * u; }
@@ -95,292 +156,262 @@ __device__ __forceinline__ void store_terms(uint16_t* h, size_t plane, size_t at
     }
 }
 
-template <bool BF, int GPC, int TERMS, int WK>
+// ---- gate | up ------------------------------------------------------------------------------------------------------
+// Block (NT tiles of gate | up, item): 16 rows of a matrix instruction, those that the item does not have as zeros, which
+// cost neither loads nor cache; WK waves take every WK-th chunk. Up to 16 rows nothing is sorted before: block (tiles, pair)
+// works if no earlier pair names its expert, a row of the instruction is the row of x, and one more block groups the pairs
+// for the launches behind.
+enum Q4Rows { ONE_ROW, FEW_ROWS, ITEMS };
+
+template <bool BF, int GPC, int TERMS, int NT, int WK, int NB, int MODE>
 __global__ void __launch_bounds__(64 * WK) q4_gateup_kernel(Q4MoeArgs a) {
-    __shared__ f4v part[WK][1][Q4_MT][64];
-    if ((int)blockIdx.y >= *a.nitems) return;
-    const Q4Item it = a.items[blockIdx.y];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t tile = blockIdx.x, chunks = q4_chunks(a.dims);
-    const uint8_t* w = a.gu + (size_t)it.expert * a.gu_bytes + (size_t)tile * chunks * q4_chunk_bytes(GPC);
-    const uint16_t* row[Q4_MT];
-    f4v out[1][Q4_MT];
-#pragma unroll
-    for (int mt = 0; mt < Q4_MT; ++mt) {
-        const int i = min(16 * mt + (lane & 15), it.count - 1);
-        row[mt] = a.x + (size_t)((uint32_t)a.sorted[it.first + i] / a.slots) * a.x_stride;
-        out[0][mt] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
-    }
-    q4_stream<BF, GPC, Q4_MT, 1, 1>(w, 0, wave, WK, chunks, row, a.dims, lane, a.sbf, out);
-#pragma unroll
-    for (int mt = 0; mt < Q4_MT; ++mt) part[wave][0][mt][lane] = out[0][mt];
-    __syncthreads();
-    for (int i = threadIdx.x; i < 128 * Q4_MT; i += 64 * WK) {
-        const int mt = i >> 7, r = (i >> 3) & 15, n = i & 7, at = 16 * mt + r;
-        const uint32_t col = tile * 8 + n;
-        if (at >= it.count || col >= a.width) continue;
-        const float v = swiglu(q4_total<WK, 1, Q4_MT>(part, 0, mt, r, n), q4_total<WK, 1, Q4_MT>(part, 0, mt, r, n + 8));
-        store_terms<TERMS>(a.h, (size_t)a.pairs * a.width, (size_t)(it.first + at) * a.width + col, v);
-    }
-}
-
-template <int GPC, int TERMS, int WK>
-__global__ void __launch_bounds__(64 * WK) q4_down_kernel(Q4MoeArgs a) {
-    __shared__ f4v part[WK][1][Q4_MT][64];
-    if ((int)blockIdx.y >= *a.nitems) return;
-    const Q4Item it = a.items[blockIdx.y];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t tile = blockIdx.x, chunks = q4_chunks(a.width);
-    const uint8_t* w = a.down + (size_t)it.expert * a.down_bytes + (size_t)tile * chunks * q4_chunk_bytes(GPC);
-    f4v out[1][Q4_MT];
-#pragma unroll
-    for (int mt = 0; mt < Q4_MT; ++mt) out[0][mt] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
-    for (uint32_t c = wave; c < chunks; c += WK) {
-        const uint8_t* p = w + (size_t)c * q4_chunk_bytes(GPC);
-        const u4v words[1] = {reinterpret_cast<const u4v*>(p)[lane]};
-        const Q4Params<GPC> par[1] = {q4_params<GPC>(p, lane)};
-#pragma unroll
-        for (int term = 0; term < TERMS; ++term) {
-            u4v x[Q4_MT][4];
-#pragma unroll
-            for (int mt = 0; mt < Q4_MT; ++mt) {
-                const int i = min(16 * mt + (lane & 15), it.count - 1);
-                q4_rows(a.h + ((size_t)term * a.pairs + it.first + i) * a.width, c, a.width, lane, x[mt]);
-            }
-            q4_chunk<true, GPC, Q4_MT, 1>(words, par, x, a.sbf, out);
-        }
-    }
-#pragma unroll
-    for (int mt = 0; mt < Q4_MT; ++mt) part[wave][0][mt][lane] = out[0][mt];
-    __syncthreads();
-    for (int i = threadIdx.x; i < 256 * Q4_MT; i += 64 * WK) {
-        const int mt = i >> 8, r = (i >> 4) & 15, n = i & 15, at = 16 * mt + r;
-        const uint32_t col = tile * 16 + n;
-        if (at >= it.count || col >= a.dims) continue;
-        a.y[(size_t)a.sorted[it.first + at] * a.dims + col] = q4_total<WK, 1, Q4_MT>(part, 0, mt, r, n);
-    }
-}
-
-__global__ void __launch_bounds__(256) q4_combine_kernel(Q4MoeArgs a) {
-    const uint32_t r = blockIdx.x, d = blockIdx.y * 256 + threadIdx.x;
-    if (d >= a.dims) return;
-    float v = 0.0f;
-    for (uint32_t k = 0; k < a.slots; ++k) {
-        const uint32_t p = r * a.slots + k;
-        if ((uint32_t)a.pick[p] < a.experts) v = __builtin_fmaf(a.wts[p], a.y[(size_t)p * a.dims + d], v);
-    }
-    store_act(a.out, a.out_dtype, (size_t)r * a.dims + d, v);
-}
-
-// ---- up to 16 rows --------------------------------------------------------------------------------------------------
-// Every distinct expert is multiplied with all rows (an MFMA takes 16 whether they are there or not), so nothing is
-// sorted: block (tiles, pair) works if no earlier pair names its expert. h is kept by pair; a row that names an expert twice
-// has it twice.
-constexpr uint32_t Q4_ROWS = 16, Q4_PAIRS = Q4_ROWS * 32;
-
-template <bool BF, int GPC, int TERMS, int NT, int WK, int NB>
-__global__ void __launch_bounds__(64 * WK) q4_gateup_rows_kernel(Q4MoeArgs a) {
     __shared__ f4v part[WK][NT][1][64];
-    __shared__ int32_t picks[Q4_PAIRS];
+    __shared__ int32_t picks[MODE == FEW_ROWS ? Q4_PAIRS : 16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t u = blockIdx.y, chunks = q4_chunks(a.dims), tiles = (a.width + 7) / 8;
-    for (uint32_t p = threadIdx.x; p < a.pairs; p += 64 * WK) picks[p] = a.pick[p];
-    __syncthreads();
-    const int32_t e = picks[u];
-    if ((uint32_t)e >= a.experts) return;
-    bool before = false;
-    for (uint32_t p = lane; p < u; p += 64) before |= picks[p] == e;
-    if (__ballot(before)) return;
-    const uint32_t first = min(blockIdx.x * NT, tiles - NT);  // the last block's tiles overlap
+    const uint32_t u = blockIdx.y, chunks = q4_chunks(a.dims), tiles = (a.width + 7) / 8, r = lane & 15;
+    int32_t e;
+    const uint16_t* row[1] = {nullptr};
+    Q4Item it{};
+    if constexpr (MODE == ONE_ROW) {  // every slot by itself: nothing is compared before the weights are read
+        e = a.pick[u];
+        if ((uint32_t)e >= a.experts) return;
+        if (r == 0) row[0] = a.x;
+    } else if constexpr (MODE == FEW_ROWS) {
+        for (uint32_t p = threadIdx.x; p < a.pairs; p += 64 * WK) picks[p] = a.pick[p];
+        __syncthreads();
+        if (u == a.pairs) {
+            if (blockIdx.x == 0) q4_group_rows<64 * WK>(a, picks);
+            return;
+        }
+        e = picks[u];
+        if ((uint32_t)e >= a.experts) return;
+        bool before = false;
+        for (uint32_t p = lane; p < u; p += 64) before |= picks[p] == e;
+        if (__ballot(before)) return;
+        if (r < a.rows)
+            for (uint32_t k = 0; k < a.slots; ++k)
+                if (picks[r * a.slots + k] == e) row[0] = a.x + (size_t)r * a.x_stride;
+    } else {
+        if ((int)u >= *a.nitems) return;
+        it = a.items[u];
+        e = it.expert;
+        const int32_t p = a.sorted[it.first + min((int)r, it.count - 1)];
+        if (threadIdx.x < 16) picks[r] = p;
+        if ((int)r < it.count) row[0] = a.x + (size_t)((uint32_t)p / a.slots) * a.x_stride;
+    }
+    const uint32_t tile0 = min(blockIdx.x * NT, tiles - NT);  // the last block's tiles overlap
     const size_t tile_bytes = (size_t)chunks * q4_chunk_bytes(GPC);
-    const uint16_t* row[1] = {a.x + (size_t)min((uint32_t)(lane & 15), a.rows - 1) * a.x_stride};
     f4v out[NT][1];
 #pragma unroll
     for (int t = 0; t < NT; ++t) out[t][0] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
-    q4_stream<BF, GPC, 1, NT, NB>(a.gu + (size_t)e * a.gu_bytes + first * tile_bytes, tile_bytes, wave, WK, chunks, row,
-                                  a.dims, lane, a.sbf, out);
+    q4_stream<BF, GPC, 1, NT, NB, true>(a.gu + (size_t)e * a.gu_bytes + tile0 * tile_bytes, tile_bytes, wave, WK, chunks, row,
+                                        a.dims, lane, a.sbf, out);
 #pragma unroll
     for (int t = 0; t < NT; ++t) part[wave][t][0][lane] = out[t][0];
     __syncthreads();
     for (int i = threadIdx.x; i < 128 * NT; i += 64 * WK) {
-        const int n = i & 7, t = (i >> 3) % NT, r = i / (8 * NT);
-        const uint32_t col = (first + t) * 8 + n;
-        if ((uint32_t)r >= a.rows || col >= a.width) continue;
-        const float v = swiglu(q4_total<WK, NT, 1>(part, t, 0, r, n), q4_total<WK, NT, 1>(part, t, 0, r, n + 8));
-        for (uint32_t k = 0; k < a.slots; ++k) {
-            const uint32_t p = r * a.slots + k;
-            if (picks[p] == e) store_terms<TERMS>(a.h, (size_t)a.pairs * a.width, (size_t)p * a.width + col, v);
+        const int n = i & 7, t = (i >> 3) % NT, m = i / (8 * NT);
+        const uint32_t col = (tile0 + t) * 8 + n;
+        uint32_t p = u;
+        bool is = col < a.width;
+        if constexpr (MODE == ONE_ROW) is = is && m == 0;
+        if constexpr (MODE == FEW_ROWS) {  // the row's first naming of the expert
+            p = m * a.slots;
+            const uint32_t end = (uint32_t)m < a.rows ? p + a.slots : p;
+            while (p < end && picks[p] != e) ++p;
+            is = is && p < end;
         }
+        if constexpr (MODE == ITEMS) {
+            p = picks[m];
+            is = is && m < it.count;
+        }
+        if (!is) continue;
+        const float v = swiglu(q4_total<WK, NT, 1>(part, t, 0, m, n), q4_total<WK, NT, 1>(part, t, 0, m, n + 8));
+        store_terms<TERMS>(a.h, (size_t)a.pairs * a.width, (size_t)p * a.width + col, v);
     }
 }
 
-// NT tiles of the output for all rows: the waves take the (distinct expert, chunk) units in turn. An activated value's terms
-// are rows of their own (term t of row r is row t * rows + r of up to 48), so few rows need one product for all terms; a
-// unit's sums are weighted into the wave's fp32 sums, and terms and waves are added at the end.
-template <int GPC, int TERMS, int MT, int NT, int WK, int NB>
-__global__ void __launch_bounds__(64 * WK) q4_down_rows_kernel(Q4MoeArgs a) {
-    __shared__ union {
-        f4v part[WK][NT][MT][64];
-        struct {
-            int32_t expert[Q4_PAIRS];
-            float weight[Q4_PAIRS][Q4_ROWS];   // [distinct][row]: the row's weight, 0 where it did not pick the expert
-            int16_t pair[Q4_PAIRS][Q4_ROWS];   // its pair, -1
-        } d;
-    } sh;
-    __shared__ int32_t picks[Q4_PAIRS];
-    __shared__ uint8_t seen[Q4_PAIRS];
-    __shared__ int ndistinct;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    static_assert(64 * WK >= Q4_PAIRS, "a thread a pair");
-    for (uint32_t p = threadIdx.x; p < a.pairs; p += 64 * WK) {
-        picks[p] = a.pick[p];
-        seen[p] = 0;
-    }
-    __syncthreads();
-    {  // whether an earlier pair names the same expert: as many threads a pair as there are
-        const uint32_t per = 64 * WK / a.pairs, p = threadIdx.x / per, sub = threadIdx.x % per;
-        if (p < a.pairs) {
-            const int32_t e = picks[p];
-            bool again = (uint32_t)e >= a.experts;
-#pragma unroll 4
-            for (uint32_t q = sub; q < p; q += per) again |= picks[q] == e;
-            if (again) seen[p] = 1;
-        }
-    }
-    __syncthreads();
-    if (wave == 0) {  // the distinct experts in the order of their first pairs
-        int n = 0;
-        for (uint32_t p0 = 0; p0 < a.pairs; p0 += 64) {
-            const bool fresh = p0 + lane < a.pairs && !seen[p0 + lane];
-            const uint64_t all = __ballot(fresh);
-            if (fresh) sh.d.expert[n + __builtin_popcountll(all & ((1ull << lane) - 1))] = picks[p0 + lane];
-            n += __builtin_popcountll(all);
-        }
-        if (lane == 0) ndistinct = n;
-    }
-    __syncthreads();
-    const int nd = ndistinct;
-    for (int i = threadIdx.x; i < nd * (int)Q4_ROWS; i += 64 * WK) {
-        const int d = i / (int)Q4_ROWS, r = i % (int)Q4_ROWS;
-        const int32_t e = sh.d.expert[d];
-        float w = 0.0f;
-        int at = -1;
-        if ((uint32_t)r < a.rows)
-            for (uint32_t k = 0; k < a.slots; ++k)
-                if (picks[r * a.slots + k] == e) {
-                    w = w + a.wts[r * a.slots + k];
-                    at = (int)(r * a.slots + k);
-                }
-        sh.d.weight[d][r] = w;
-        sh.d.pair[d][r] = (int16_t)at;
-    }
-    __syncthreads();
-    const uint32_t chunks = q4_chunks(a.width), tiles = q4_tiles(a.dims), first = min(blockIdx.x * NT, tiles - NT);
-    const size_t tile_bytes = (size_t)chunks * q4_chunk_bytes(GPC), plane = (size_t)a.pairs * a.width;
-    const uint8_t* w0 = a.down + first * tile_bytes;
-    f4v out[NT][MT];
+// ---- down -----------------------------------------------------------------------------------------------------------
+// One row: NT tiles of the output a block; its waves take the (slot, chunk) units in turn, weigh their sums in registers, and
+// terms (rows 0 .. TERMS - 1 of the instruction) and waves are added at the end.
+template <int GPC, int TERMS, int NT, int WK, int NB>
+__global__ void __launch_bounds__(64 * WK) q4_down_one_kernel(Q4MoeArgs a) {
+    __shared__ f4v part[WK][NT][1][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), term = lane & 15;
+    const uint32_t chunks = q4_chunks(a.width), tiles = q4_tiles(a.dims), units = a.slots * chunks;
+    const uint32_t tile0 = min(blockIdx.x * NT, tiles - NT);
+    const size_t tile_bytes = (size_t)chunks * q4_chunk_bytes(GPC), plane = (size_t)a.slots * a.width;
+    f4v out[NT];
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) out[t][mt] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
-    // the lane's rows: as A operand, row 16 mt + (lane & 15); in the sums, rows 16 mt + 4 (lane >> 4) + i
-    const uint32_t units = nd * chunks;
+    for (int t = 0; t < NT; ++t) out[t] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
     for (uint32_t u0 = wave; u0 < units; u0 += WK * NB) {
-        u4v words[NB][NT], x[NB][MT][4];
+        u4v words[NB][NT], x[NB][1][4];
         Q4Params<GPC> par[NB][NT];
+        int32_t e[NB];
+        float w[NB];
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
-            const uint32_t u = min(u0 + WK * i, units - 1), d = u / chunks, c = u - d * chunks;
-            const uint8_t* p = w0 + (size_t)sh.d.expert[d] * a.down_bytes + (size_t)c * q4_chunk_bytes(GPC);
+            const uint32_t slot = min(u0 + WK * i, units - 1) / chunks;
+            e[i] = a.pick[slot];
+            w[i] = a.wts[slot];
+        }
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            const uint32_t u = min(u0 + WK * i, units - 1), c = u % chunks;
+            const uint8_t* p = a.down + (size_t)((uint32_t)e[i] < a.experts ? e[i] : 0) * a.down_bytes + tile0 * tile_bytes +
+                               (size_t)c * q4_chunk_bytes(GPC);
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 words[i][t] = reinterpret_cast<const u4v*>(p + t * tile_bytes)[lane];
                 par[i][t] = q4_params<GPC>(p + t * tile_bytes, lane);
             }
+        }
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                const uint32_t v = 16 * mt + (lane & 15), term = v / a.rows;
-                const int at = term < TERMS ? sh.d.pair[d][v - term * a.rows] : -1;
+        for (int i = 0; i < NB; ++i)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) x[i][mt][j] = u4v{0, 0, 0, 0};
-                if (at >= 0) q4_rows(a.h + term * plane + (size_t)at * a.width, c, a.width, lane, x[i][mt]);
+            for (int j = 0; j < 4; ++j) x[i][0][j] = u4v{0, 0, 0, 0};
+        if (term < TERMS) {
+#pragma unroll
+            for (int i = 0; i < NB; ++i) {
+                const uint32_t u = min(u0 + WK * i, units - 1);
+                q4_rows(a.h + term * plane + (size_t)(u / chunks) * a.width, u % chunks, a.width, lane, x[i][0]);
             }
         }
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
-            if (u0 + WK * i >= units) break;
-            const uint32_t d = (u0 + WK * i) / chunks;
-            f4v y[NT][MT];
+            if (u0 + WK * i >= units || (uint32_t)e[i] >= a.experts) continue;
+            f4v y[NT][1];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) y[t][0] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+            q4_chunk<true, GPC, 1, NT>(words[i], par[i], x[i], a.sbf, y);
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) y[t][mt] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
-            q4_chunk<true, GPC, MT, NT>(words[i], par[i], x[i], a.sbf, y);
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const uint32_t v = 16 * mt + 4 * (lane >> 4) + r, term = v / a.rows;
-                    const float wt = term < TERMS ? sh.d.weight[d][v - term * a.rows] : 0.0f;
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) out[t][mt][r] = __builtin_fmaf(wt, y[t][mt][r], out[t][mt][r]);
-                }
+                for (int r = 0; r < TERMS; ++r) out[t][r] = __builtin_fmaf(w[i], y[t][0][r], out[t][r]);
         }
     }
-    __syncthreads();  // the tables are done with
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) sh.part[wave][t][mt][lane] = out[t][mt];
+    for (int t = 0; t < NT; ++t) part[wave][t][0][lane] = out[t];
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < 16 * NT * a.rows; i += 64 * WK) {
-        const int n = i & 15, t = (i >> 4) % NT;
-        const uint32_t r = i / (16 * NT), col = (first + t) * 16 + n;
+    for (int i = threadIdx.x; i < 16 * NT; i += 64 * WK) {
+        const int n = i & 15, t = i >> 4;
+        const uint32_t col = (tile0 + t) * 16 + n;
         if (col >= a.dims) continue;
-        float v = 0.0f;
+        float v = q4_total<WK, NT, 1>(part, t, 0, TERMS - 1, n);
 #pragma unroll
-        for (int k = TERMS - 1; k >= 0; --k) {  // the small terms first
-            const uint32_t vr = k * a.rows + r;
-            v = v + q4_total<WK, NT, MT>(sh.part, t, vr >> 4, vr & 15, n);
-        }
-        store_act(a.out, a.out_dtype, (size_t)r * a.dims + col, v);
+        for (int r = TERMS - 2; r >= 0; --r) v = v + q4_total<WK, NT, 1>(part, t, 0, r, n);  // the small terms first
+        store_act(a.out, a.out_dtype, col, v);
     }
 }
 
-template <int GPC, int TERMS>
-static void launch_rows(hipStream_t s, const Q4MoeArgs& a, bool bf) {
-    const unsigned tiles = (a.width + 7) / 8, dtiles = q4_tiles(a.dims);
-    auto gateup = [&](auto bf_) {
-        constexpr bool BF = decltype(bf_)::value;
-        if (a.rows <= 4 || tiles < 2) q4_gateup_rows_kernel<BF, GPC, TERMS, 1, 8, 3><<<dim3(tiles, a.pairs), 512, 0, s>>>(a);
-        else q4_gateup_rows_kernel<BF, GPC, TERMS, 2, 8, 3><<<dim3((tiles + 1) / 2, a.pairs), 512, 0, s>>>(a);
-    };
-    if (bf) gateup(std::true_type{});
-    else gateup(std::false_type{});
-    auto down = [&](auto mt_) {
-        constexpr int MT = decltype(mt_)::value;
-        q4_down_rows_kernel<GPC, TERMS, MT, 1, 8, 2><<<dtiles, 512, 0, s>>>(a);
-    };
-    const uint32_t groups = (a.rows * TERMS + 15) / 16;
-    if (groups == 1) down(std::integral_constant<int, 1>{});
-    else if (TERMS > 1 && groups == 2) down(std::integral_constant<int, TERMS < 2 ? 1 : 2>{});
-    else down(std::integral_constant<int, TERMS>{});
+// More rows: block (WK NT tiles, item), a wave its NT tiles over all of the width, so that no sum crosses waves and an
+// expert's weights are read where they lie together (blocks that took some tiles of every expert read them at half the rate).
+// Terms are rows of their own: rows 4 q .. 4 q + 3 of the instruction are quad q of the accumulators' lanes; with three
+// terms quad q holds term q of four pairs, with two quads 2 q and 2 q + 1 term q of eight, and adding lanes 16 (and 32)
+// apart adds the terms.
+template <int GPC, int TERMS, int NT, int WK, int NB>
+__global__ void __launch_bounds__(64 * WK) q4_down_kernel(Q4MoeArgs a) {
+    constexpr int PER = TERMS == 1 ? 16 : TERMS == 2 ? 8 : 4;  // pairs a product
+    if ((int)blockIdx.y >= *a.nitems) return;
+    const Q4Item it = a.items[blockIdx.y];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t chunks = q4_chunks(a.width), tiles = q4_tiles(a.dims), mine = (blockIdx.x * WK + wave) * NT;
+    if (mine >= tiles) return;
+    const uint32_t tile0 = min(mine, tiles - NT);  // the last wave's tiles overlap
+    const size_t tile_bytes = (size_t)chunks * q4_chunk_bytes(GPC), plane = (size_t)a.pairs * a.width;
+    const uint8_t* w = a.down + (size_t)it.expert * a.down_bytes + tile0 * tile_bytes;
+    for (int m0 = 0; m0 < it.count; m0 += PER) {
+        const int m = m0 + (lane & (PER - 1)), term = (lane & 15) / PER;
+        const uint16_t* row[1] = {nullptr};
+        if (m < it.count && term < TERMS) row[0] = a.h + term * plane + (size_t)a.sorted[it.first + m] * a.width;
+        f4v out[NT][1];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) out[t][0] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+        q4_stream<true, GPC, 1, NT, NB, true>(w, tile_bytes, 0, 1, chunks, row, a.width, lane, a.sbf, out);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int q = lane >> 4, at = m0 + 4 * (q & (PER / 4 - 1)) + i;  // the pair of this quad's value i
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                float v = out[t][0][i];
+                if constexpr (TERMS == 3) v = v + lane_xor<16>(v);
+                if constexpr (TERMS >= 2) v = v + lane_xor<32>(v);
+                const uint32_t col = (tile0 + t) * 16 + (lane & 15);
+                if (at < it.count && q < PER / 4 && col < a.dims)
+                    a.y[(size_t)a.sorted[it.first + at] * a.dims + col] = v;
+            }
+        }
+    }
 }
 
+// ---- a row's slots, in order ----------------------------------------------------------------------------------------
+__global__ void __launch_bounds__(256) q4_combine_kernel(Q4MoeArgs a) {
+    __shared__ int32_t pick[32];
+    __shared__ float weight[32];
+    const uint32_t r = blockIdx.x, d = blockIdx.y * 256 + threadIdx.x;
+    if (threadIdx.x < a.slots) pick[threadIdx.x] = a.pick[(size_t)r * a.slots + threadIdx.x];
+    __syncthreads();
+    if (threadIdx.x < a.slots) {  // an expert named again adds its weight to the first naming
+        const int32_t e = pick[threadIdx.x];
+        bool first = (uint32_t)e < a.experts;
+        float w = 0.0f;
+        for (uint32_t k = 0; k < a.slots; ++k) {
+            first = first && !(k < threadIdx.x && pick[k] == e);
+            if (k >= threadIdx.x && pick[k] == e) w = w + a.wts[(size_t)r * a.slots + k];
+        }
+        weight[threadIdx.x] = w;
+        __builtin_amdgcn_wave_barrier();
+        if (!first) pick[threadIdx.x] = -1;
+    }
+    __syncthreads();
+    if (d >= a.dims) return;
+    float v = 0.0f;
+    for (uint32_t k = 0; k < a.slots; ++k)
+        if (pick[k] >= 0) v = __builtin_fmaf(weight[k], a.y[((size_t)r * a.slots + k) * a.dims + d], v);
+    store_act(a.out, a.out_dtype, (size_t)r * a.dims + d, v);
+}
+
+// ---- launches -------------------------------------------------------------------------------------------------------
 template <int GPC, int TERMS>
-static void launch_items(hipStream_t s, const Q4MoeArgs& a, bool bf, uint32_t max_items) {
-    const dim3 gu((a.width + 7) / 8, max_items), dn((a.dims + 15) / 16, max_items);
-    if (bf) q4_gateup_kernel<true, GPC, TERMS, 4><<<gu, 256, 0, s>>>(a);
-    else q4_gateup_kernel<false, GPC, TERMS, 4><<<gu, 256, 0, s>>>(a);
-    q4_down_kernel<GPC, TERMS, 2><<<dn, 128, 0, s>>>(a);
+static void launch_moe(hipStream_t s, const Q4MoeArgs& a, bool bf, uint32_t max_items) {
+    const uint32_t tiles = (a.width + 7) / 8, dtiles = q4_tiles(a.dims);
+    auto gateup = [&](auto bf_, auto nt_, auto mode_, uint32_t blocks) {
+        constexpr int NT = decltype(nt_)::value, WK = 8;
+        q4_gateup_kernel<decltype(bf_)::value, GPC, TERMS, NT, WK, 3, decltype(mode_)::value>
+            <<<dim3((tiles + NT - 1) / NT, blocks), 64 * WK, 0, s>>>(a);
+    };
+    auto with = [&](auto nt_, auto mode_, uint32_t blocks) {
+        if (bf) gateup(std::true_type{}, nt_, mode_, blocks);
+        else gateup(std::false_type{}, nt_, mode_, blocks);
+    };
+    using One = std::integral_constant<int, 1>;
+    using Two = std::integral_constant<int, 2>;
+    if (a.rows == 1) {
+        with(One{}, std::integral_constant<int, ONE_ROW>{}, a.pairs);
+        q4_down_one_kernel<GPC, TERMS, 1, 8, 2><<<dtiles, 512, 0, s>>>(a);
+        return;
+    }
+    if (a.rows <= Q4_ROWS) {
+        const std::integral_constant<int, FEW_ROWS> few{};
+        if (a.rows <= 4 || tiles < 2) with(One{}, few, a.pairs + 1);
+        else with(Two{}, few, a.pairs + 1);
+    } else {
+        q4_group_kernel<<<1, 1024, 0, s>>>(a);
+        const std::integral_constant<int, ITEMS> items{};
+        if (tiles < 2) with(One{}, items, max_items);
+        else with(Two{}, items, max_items);
+    }
+    if (dtiles >= 4) q4_down_kernel<GPC, TERMS, 4, 4, 2><<<dim3((dtiles + 15) / 16, max_items), 256, 0, s>>>(a);
+    else q4_down_kernel<GPC, TERMS, 1, 4, 2><<<dim3((dtiles + 3) / 4, max_items), 256, 0, s>>>(a);
+    q4_combine_kernel<<<dim3(a.rows, (a.dims + 255) / 256), 256, 0, s>>>(a);
 }
 
 // Terms of the activated values: what the output's type can show (bf16 8 bits, fp16 11, fp32 24).
 static int q4_terms(int out_dtype) { return out_dtype == BF16 ? 1 : out_dtype == F16 ? 2 : 3; }
 
 static uint32_t q4_max_items(uint32_t experts, size_t pairs) {
-    const size_t full = pairs / (16 * Q4_MT), some = pairs < experts ? pairs : experts;
+    const size_t full = pairs / Q4_ITEM, some = pairs < experts ? pairs : experts;
     return (uint32_t)(full + some);
 }
 
@@ -422,7 +453,7 @@ extern "C" {
 
 size_t ea_q4_scratch_bytes(const ea_q4_experts* ex, uint32_t rows, uint32_t slots) {
     ea_q4_scratch s;
-    if (q4_experts_ok(ex) || rows == 0 || rows > EA_Q4_MAX_ROWS || slots == 0 || slots > 32) return 0;
+    if (q4_experts_ok(ex) || rows == 0 || slots == 0 || slots > 32 || (uint64_t)rows * slots > EA_Q4_MAX_PAIRS) return 0;
     return q4_carve(&s, 0, ex, rows, slots);
 }
 
@@ -430,8 +461,9 @@ int ea_q4_scratch_init(ea_q4_scratch* s, void* base, size_t bytes, const ea_q4_e
                        uint32_t slots) {
     int r = q4_experts_ok(ex);
     if (r) return r;
-    if (!s || !base || (reinterpret_cast<uintptr_t>(base) & 255) || rows == 0 || rows > EA_Q4_MAX_ROWS) return EA_BAD_ARGUMENT;
+    if (!s || !base || (reinterpret_cast<uintptr_t>(base) & 255) || rows == 0) return EA_BAD_ARGUMENT;
     if (slots == 0 || slots > 32) return EA_TOO_MANY_SLOTS;
+    if ((uint64_t)rows * slots > EA_Q4_MAX_PAIRS) return EA_BAD_ARGUMENT;
     if (bytes < ea_q4_scratch_bytes(ex, rows, slots)) return EA_SCRATCH_TOO_SMALL;
     q4_carve(s, (uint64_t)reinterpret_cast<uintptr_t>(base), ex, rows, slots);
     s->experts = ex->count;
@@ -478,29 +510,15 @@ int ea_q4_routed(ea_stream_t stream, const void* x, int x_dtype, uint32_t x_stri
     a.sbf = ex->s_dtype == BF16;
     const uint32_t max_items = q4_max_items(a.experts, a.pairs);
     hipStream_t s = as_stream(stream);
-    if (R <= Q4_ROWS) {
-        auto go = [&](auto gpc_) {
-            constexpr int GPC = decltype(gpc_)::value;
-            if (terms == 1) launch_rows<GPC, 1>(s, a, x_dtype == BF16);
-            else if (terms == 2) launch_rows<GPC, 2>(s, a, x_dtype == BF16);
-            else launch_rows<GPC, 3>(s, a, x_dtype == BF16);
-        };
-        if (gpc == 4) go(std::integral_constant<int, 4>{});
-        else if (gpc == 2) go(std::integral_constant<int, 2>{});
-        else go(std::integral_constant<int, 1>{});
-        return launched();
-    }
-    q4_group_kernel<<<1, 1024, 0, s>>>(a);
     auto go = [&](auto gpc_) {
         constexpr int GPC = decltype(gpc_)::value;
-        if (terms == 1) launch_items<GPC, 1>(s, a, x_dtype == BF16, max_items);
-        else if (terms == 2) launch_items<GPC, 2>(s, a, x_dtype == BF16, max_items);
-        else launch_items<GPC, 3>(s, a, x_dtype == BF16, max_items);
+        if (terms == 1) launch_moe<GPC, 1>(s, a, x_dtype == BF16, max_items);
+        else if (terms == 2) launch_moe<GPC, 2>(s, a, x_dtype == BF16, max_items);
+        else launch_moe<GPC, 3>(s, a, x_dtype == BF16, max_items);
     };
     if (gpc == 4) go(std::integral_constant<int, 4>{});
     else if (gpc == 2) go(std::integral_constant<int, 2>{});
     else go(std::integral_constant<int, 1>{});
-    q4_combine_kernel<<<dim3(R, (a.dims + 255) / 256), 256, 0, s>>>(a);
     return launched();
 }
 

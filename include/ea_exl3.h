@@ -308,7 +308,8 @@ int ea_route(ea_stream_t stream, const void* logits, int l_dtype, uint32_t l_str
  * EXL3-encoded. The products take x as it is (fp16 or bf16), multiply by the integers q and apply scale and bias to fp32
  * sums of a group, so no weight is rounded; a group's bias times its sum of x is added apart, so a row with an infinity
  * gives infinities or NaN in all of its outputs. */
-#define EA_Q4_MAX_ROWS 65536
+#define EA_Q4_MAX_ROWS 65536    /* of a linear's call */
+#define EA_Q4_MAX_PAIRS 524288  /* rows * slots of the experts' */
 
 /* Bytes of one packed matrix [n, k]; 0 for a group other than 32, 64 or 128, k % group != 0, or n or k 0. */
 size_t ea_q4_bytes(uint32_t n, uint32_t k, uint32_t group);
@@ -350,7 +351,7 @@ size_t ea_q4_scratch_bytes(const ea_q4_experts* ex, uint32_t rows, uint32_t slot
 int ea_q4_scratch_init(ea_q4_scratch* s, void* base, size_t bytes, const ea_q4_experts* ex, uint32_t rows, uint32_t slots);
 
 /* out [R, dims] (fp16, bf16 or fp32) = sum over the slots of wts * down(silu(gate(x)) * up(x)) of the picked experts: what
- * ea_moe_routed and ea_prompt_experts_run are for EXL3 experts, for one row to EA_Q4_MAX_ROWS. pick int32 / wts fp32
+ * ea_moe_routed and ea_prompt_experts_run are for EXL3 experts, for one row to a whole prompt's (EA_Q4_MAX_PAIRS). pick int32 / wts fp32
  * [R, slots] (slots: the scratch's); a pick outside 0 .. count - 1 is a slot without an expert, a row of such picks gives
  * zeros, and a row may name an expert twice. The activated values are held as one, two or three bf16 numbers that add up to
  * them, as many as out's type can show. The same bits on every run. EA_SCRATCH_TOO_SMALL: R above the scratch's rows, or a

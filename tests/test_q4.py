@@ -81,7 +81,7 @@ def test_experts_refuse():
     init = lambda e=ex, base=4096, size=n, rows=8, slots=2: L.ea_q4_scratch_init(  # noqa: E731
         C.byref(sc), base, size, C.byref(e), rows, slots)
     assert init(size=n - 1) == 12 and init(base=0) == 18 and init(base=4097) == 18 and init(slots=33) == 6
-    assert init(slots=0) == 6 and init(rows=0) == 18 and init(rows=65537, size=1 << 60) == 18
+    assert init(slots=0) == 6 and init(rows=0) == 18 and init(rows=262145, size=1 << 60) == 18
     for e, code in ((_ex(group=48), 11), (_ex(dims=224), 8), (_ex(width=96), 8), (_ex(count=0), 18), (_ex(count=4097), 5),
                     (_ex(gu=0), 18), (_ex(down=0), 18), (_ex(s_dtype=2), 18), (_ex(dims=0), 18)):
         assert init(e) == code
