@@ -71,11 +71,10 @@ struct Q4LinArgs {
     size_t x_stride;
     uint32_t m, k, chunks;
     int jobs;
-    bool sbf;
 };
 
 // A block takes NT tiles of one job and 16 MT rows; its WK waves take every WK-th chunk and add their sums in wave order.
-template <bool BF, int GPC, int MT, int NT, int WK, int NB>
+template <bool BF, bool SBF, int GPC, int MT, int NT, int WK, int NB>
 __global__ void __launch_bounds__(64 * WK) q4_linear_kernel(Q4LinArgs a) {
     __shared__ f4v part[WK][NT][MT][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -92,8 +91,8 @@ __global__ void __launch_bounds__(64 * WK) q4_linear_kernel(Q4LinArgs a) {
 #pragma unroll
         for (int t = 0; t < NT; ++t) out[t][mt] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    q4_stream<BF, GPC, MT, NT, NB>(job.w + first * tile_bytes, tiles < NT ? 0 : tile_bytes, wave, WK, a.chunks, row, a.k, lane,
-                                   a.sbf, out);
+    q4_stream<BF, SBF, GPC, MT, NT, NB>(job.w + first * tile_bytes, tiles < NT ? 0 : tile_bytes, wave, WK, a.chunks, row, a.k, lane,
+                                   out);
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -107,23 +106,17 @@ __global__ void __launch_bounds__(64 * WK) q4_linear_kernel(Q4LinArgs a) {
     }
 }
 
-static int launch_linear(hipStream_t s, const Q4LinArgs& a, uint32_t tiles, bool bf, int gpc) {
-    auto go = [&](auto gpc_, auto bf_) {
+static int launch_linear(hipStream_t s, const Q4LinArgs& a, uint32_t tiles, bool bf, bool sbf, int gpc) {
+    auto go = [&](auto gpc_, auto bf_, auto sbf_) {
         constexpr int GPC = decltype(gpc_)::value;
-        constexpr bool BF = decltype(bf_)::value;
+        constexpr bool BF = decltype(bf_)::value, SBF = decltype(sbf_)::value;
         const unsigned jobs = (unsigned)a.jobs;
         if (a.m <= 16) {
-            if (tiles * jobs < 512) q4_linear_kernel<BF, GPC, 1, 1, 16, 3><<<dim3(tiles, 1, jobs), 1024, 0, s>>>(a);
-            else q4_linear_kernel<BF, GPC, 1, 2, 8, 3><<<dim3((tiles + 1) / 2, 1, jobs), 512, 0, s>>>(a);
-        } else q4_linear_kernel<BF, GPC, 4, 1, 8, 1><<<dim3(tiles, (a.m + 63) / 64, jobs), 512, 0, s>>>(a);
+            if (tiles * jobs < 512) q4_linear_kernel<BF, SBF, GPC, 1, 1, 16, 3><<<dim3(tiles, 1, jobs), 1024, 0, s>>>(a);
+            else q4_linear_kernel<BF, SBF, GPC, 1, 2, 8, 3><<<dim3((tiles + 1) / 2, 1, jobs), 512, 0, s>>>(a);
+        } else q4_linear_kernel<BF, SBF, GPC, 4, 1, 8, 1><<<dim3(tiles, (a.m + 63) / 64, jobs), 512, 0, s>>>(a);
     };
-    auto go_g = [&](auto bf_) {
-        if (gpc == 4) go(std::integral_constant<int, 4>{}, bf_);
-        else if (gpc == 2) go(std::integral_constant<int, 2>{}, bf_);
-        else go(std::integral_constant<int, 1>{}, bf_);
-    };
-    if (bf) go_g(std::true_type{});
-    else go_g(std::false_type{});
+    q4_types(bf, sbf, gpc, go);
     return launched();
 }
 
@@ -192,8 +185,7 @@ int ea_q4_call(ea_stream_t stream, const ea_q4_linear* const* ls, uint32_t nls, 
     a.k = ls[0]->k;
     a.chunks = q4_chunks(a.k);
     a.jobs = (int)nls;
-    a.sbf = ls[0]->s_dtype == BF16;
-    return launch_linear(as_stream(stream), a, tiles, x_dtype == BF16, 128 / (int)ls[0]->group);
+    return launch_linear(as_stream(stream), a, tiles, x_dtype == BF16, ls[0]->s_dtype == BF16, 128 / (int)ls[0]->group);
 }
 
 }  // extern "C"

@@ -12,6 +12,8 @@
 
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "ea_device.hpp"
 
 namespace ea {
@@ -65,17 +67,18 @@ template <int GPC>
 __device__ __forceinline__ Q4Params<GPC> q4_params(const uint8_t* chunk, int lane) {
     return *reinterpret_cast<const Q4Params<GPC>*>(chunk + Q4_WORDS + 4 * GPC * (lane & 15));
 }
-__device__ __forceinline__ void q4_scale_bias(uint32_t p, bool bf, float& s, float& b) {
-    s = bf ? __builtin_bit_cast(float, p << 16) : h2f((uint16_t)(p & 0xffffu));
-    b = bf ? __builtin_bit_cast(float, p & 0xffff0000u) : h2f((uint16_t)(p >> 16));
+template <bool SBF>
+__device__ __forceinline__ void q4_scale_bias(uint32_t p, float& s, float& b) {
+    s = SBF ? __builtin_bit_cast(float, p << 16) : h2f((uint16_t)(p & 0xffffu));
+    b = SBF ? __builtin_bit_cast(float, p & 0xffff0000u) : h2f((uint16_t)(p >> 16));
 }
 
 // A chunk of NT tiles against MT groups of 16 rows: out += the chunk's share. a[mt][j]: the rows' A operands of the chunk's
 // four products. The sums of x come from the same operands against ones, which leaves them in the accumulators' own layout
 // (lane l: rows 4 (l >> 4) + i, weight row l & 15).
-template <bool BF, int GPC, int MT, int NT>
+template <bool BF, bool SBF, int GPC, int MT, int NT>
 __device__ __forceinline__ void q4_chunk(const u4v (&words)[NT], const Q4Params<GPC> (&par)[NT], const u4v (&a)[MT][4],
-                                         bool sbf, f4v (&out)[NT][MT]) {
+                                         f4v (&out)[NT][MT]) {
     constexpr int JPG = 4 / GPC;
     const f4v zero{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -95,7 +98,7 @@ __device__ __forceinline__ void q4_chunk(const u4v (&words)[NT], const Q4Params<
                 for (int mt = 0; mt < MT; ++mt) acc[mt] = q4_mfma<BF>(a[mt][g * JPG + j], b, j ? acc[mt] : zero);
             }
             float s, b;
-            q4_scale_bias(par[t].w[g], sbf, s, b);
+            q4_scale_bias<SBF>(par[t].w[g], s, b);
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -116,9 +119,9 @@ __device__ __forceinline__ void q4_rows(const uint16_t* row, uint32_t chunk, uin
 
 // The tiles at w, w + tile_bytes, .. against MT groups of 16 rows over the chunks c0, c0 + step, ..: the loads of NB chunks
 // are issued before the first of their products. With SOME, a lane whose row is null reads nothing and multiplies zeros.
-template <bool BF, int GPC, int MT, int NT, int NB, bool SOME = false>
+template <bool BF, bool SBF, int GPC, int MT, int NT, int NB, bool SOME = false>
 __device__ __forceinline__ void q4_stream(const uint8_t* w, size_t tile_bytes, uint32_t c0, uint32_t step, uint32_t chunks,
-                                          const uint16_t* const (&row)[MT], uint32_t k, int lane, bool sbf,
+                                          const uint16_t* const (&row)[MT], uint32_t k, int lane,
                                           f4v (&out)[NT][MT]) {
     for (uint32_t c = c0; c < chunks; c += step * NB) {
         u4v words[NB][NT], x[NB][MT][4];
@@ -150,7 +153,7 @@ __device__ __forceinline__ void q4_stream(const uint8_t* w, size_t tile_bytes, u
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < NB; ++i)
-            if (c + step * i < chunks) q4_chunk<BF, GPC, MT, NT>(words[i], par[i], x[i], sbf, out);
+            if (c + step * i < chunks) q4_chunk<BF, SBF, GPC, MT, NT>(words[i], par[i], x[i], out);
     }
 }
 
@@ -162,6 +165,20 @@ __device__ __forceinline__ float q4_total(const f4v (&part)[WK][NT][MT][64], int
 #pragma unroll
     for (int k = 1; k < WK; ++k) v = v + all[k * NT * MT * 256];
     return v;
+}
+
+// f(groups a chunk, x in bf16, scales in bf16) as compile-time constants.
+template <typename F>
+inline void q4_types(bool bf, bool sbf, int gpc, F f) {
+    const auto types = [&](auto gpc_) {
+        if (bf && sbf) f(gpc_, std::true_type{}, std::true_type{});
+        else if (bf) f(gpc_, std::true_type{}, std::false_type{});
+        else if (sbf) f(gpc_, std::false_type{}, std::true_type{});
+        else f(gpc_, std::false_type{}, std::false_type{});
+    };
+    if (gpc == 4) types(std::integral_constant<int, 4>{});
+    else if (gpc == 2) types(std::integral_constant<int, 2>{});
+    else types(std::integral_constant<int, 1>{});
 }
 
 }  // namespace ea

@@ -18,8 +18,10 @@ constexpr uint32_t Q4_MAX_EXPERTS = 4096;
 constexpr uint32_t Q4_ITEM = 16;                       // rows an item
 constexpr uint32_t Q4_ROWS = 16, Q4_PAIRS = Q4_ROWS * 32;  // rows and pairs that are grouped beside the first products
 
+// An expert and up to 16 of its pairs (row * slots + slot).
 struct Q4Item {
-    int32_t expert, first, count, pad;
+    int32_t expert, count;
+    int32_t pair[Q4_ITEM];
 };
 
 struct Q4MoeArgs {
@@ -29,57 +31,71 @@ struct Q4MoeArgs {
     const float* wts;
     const uint8_t *gu, *down;
     size_t gu_bytes, down_bytes;  // one expert's
-    int32_t *sorted, *nitems;     // pairs by expert; the number of items
-    Q4Item* items;                // runs of sorted
+    int32_t* nitems;
+    Q4Item* items;
     uint16_t* h;                  // bf16 [terms][pairs][width]
     float* y;                     // fp32 [pairs][dims]
     void* out;
     uint32_t rows, pairs, dims, width, experts, slots;
-    int out_dtype;
-    bool sbf;
+    int out_dtype, terms;
 };
 
 // ---- grouping -----------------------------------------------------------------------------------------------------
-// One block: the pairs of each expert counted, the counts scanned, the pairs placed (in any order within an expert), the
-// items listed. A pick outside 0 .. experts - 1 is a slot without an expert.
+// One block: the pairs of each expert counted, the items before each expert scanned, the pairs placed (in any order within an
+// expert). A pick outside 0 .. experts - 1 is a slot without an expert.
 __global__ void __launch_bounds__(1024) q4_group_kernel(Q4MoeArgs a) {
-    __shared__ uint32_t count[Q4_MAX_EXPERTS], start[Q4_MAX_EXPERTS], sums[2][16];
+    __shared__ uint32_t count[Q4_MAX_EXPERTS], start[Q4_MAX_EXPERTS], sums[16];
+    constexpr int KEEP = 8;  // picks a thread keeps between the passes
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    uint32_t kept[KEEP];
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i) kept[i] = (uint32_t)(t + 1024u * i) < a.pairs ? (uint32_t)a.pick[t + 1024 * i] : 0xffffffffu;
     for (uint32_t e = t; e < a.experts; e += 1024) count[e] = 0;
     __syncthreads();
-    for (uint32_t p = t; p < a.pairs; p += 1024) {
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i)
+        if (kept[i] < a.experts) atomicAdd(&count[kept[i]], 1u);
+    for (uint32_t p = t + 1024 * KEEP; p < a.pairs; p += 1024) {
         const uint32_t e = (uint32_t)a.pick[p];
         if (e < a.experts) atomicAdd(&count[e], 1u);
     }
     __syncthreads();
-    // exclusive scans of the counts and the item counts, 1024 experts a step
-    uint32_t base = 0, ibase = 0;
-    for (uint32_t e0 = 0; e0 < a.experts; e0 += 1024) {
+    uint32_t base = 0;
+    for (uint32_t e0 = 0; e0 < a.experts; e0 += 1024) {  // an exclusive scan of the experts' items, 1024 experts a step
         const uint32_t e = e0 + t, c = e < a.experts ? count[e] : 0, n = (c + Q4_ITEM - 1) / Q4_ITEM;
-        uint32_t v = c, w = n;
+        uint32_t v = n;
         for (int d = 1; d < 64; d <<= 1) {
-            const uint32_t pv = __shfl_up(v, d), pw = __shfl_up(w, d);
-            if (lane >= d) v += pv, w += pw;
+            const uint32_t o = __shfl_up(v, d);
+            v += lane >= d ? o : 0;
         }
-        if (lane == 63) sums[0][wave] = v, sums[1][wave] = w;
+        if (lane == 63) sums[wave] = v;
         __syncthreads();
-        uint32_t bv = base, bw = ibase;
+        uint32_t item = base + v - n;
         for (int i = 0; i < 16; ++i) {
-            const uint32_t sv = sums[0][i], sw = sums[1][i];
-            if (i < wave) bv += sv, bw += sw;
-            base += sv;
-            ibase += sw;
+            item += i < wave ? sums[i] : 0;
+            base += sums[i];
         }
-        const uint32_t first = bv + v - c, item = bw + w - n;
-        if (e < a.experts) start[e] = first;
-        for (uint32_t i = 0; i < n; ++i)
-            a.items[item + i] = Q4Item{(int32_t)e, (int32_t)(first + i * Q4_ITEM), (int32_t)min(c - i * Q4_ITEM, Q4_ITEM), 0};
+        if (e < a.experts) {
+            start[e] = item;
+            count[e] = 0;
+        }
+        for (uint32_t i = 0; i < n; ++i) {
+            a.items[item + i].expert = (int32_t)e;
+            a.items[item + i].count = (int32_t)min(c - i * Q4_ITEM, Q4_ITEM);
+        }
         __syncthreads();
     }
-    if (t == 0) *a.nitems = (int32_t)ibase;
-    for (uint32_t p = t; p < a.pairs; p += 1024) {
+    if (t == 0) *a.nitems = (int32_t)base;
+    const auto place = [&](uint32_t p, uint32_t e) {
+        const uint32_t at = atomicAdd(&count[e], 1u);
+        a.items[start[e] + at / Q4_ITEM].pair[at % Q4_ITEM] = (int32_t)p;
+    };
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i)
+        if (kept[i] < a.experts) place(t + 1024 * i, kept[i]);
+    for (uint32_t p = t + 1024 * KEEP; p < a.pairs; p += 1024) {
         const uint32_t e = (uint32_t)a.pick[p];
-        if (e < a.experts) a.sorted[atomicAdd(&start[e], 1u)] = (int32_t)p;
+        if (e < a.experts) place(p, e);
     }
 }
 
@@ -88,68 +104,61 @@ __global__ void __launch_bounds__(1024) q4_group_kernel(Q4MoeArgs a) {
 // weight to the first naming.
 template <int THREADS>
 __device__ void q4_group_rows(const Q4MoeArgs& a, int32_t* picks) {
-    __shared__ int16_t owner[Q4_PAIRS], before[Q4_PAIRS], count[Q4_PAIRS], first[Q4_PAIRS];
+    __shared__ int16_t owner[Q4_PAIRS], before[Q4_PAIRS], index[Q4_PAIRS];
     int32_t once[(Q4_PAIRS + THREADS - 1) / THREADS];
     for (uint32_t p = threadIdx.x, i = 0; p < a.pairs; p += THREADS, ++i) {
         int32_t e = picks[p];
         e = (uint32_t)e < a.experts ? e : -1;
         for (uint32_t q = p - p % a.slots; q < p; ++q) e = picks[q] == e ? -1 : e;
         once[i] = e;
-        count[p] = 0;
     }
     __syncthreads();
     for (uint32_t p = threadIdx.x, i = 0; p < a.pairs; p += THREADS, ++i) picks[p] = once[i];
     __syncthreads();
     for (uint32_t p = threadIdx.x; p < a.pairs; p += THREADS) {
         const int32_t e = picks[p];
-        uint32_t n = 0, own = p, all = 0;
+        uint32_t n = 0, own = p;
         if (e >= 0) {
 #pragma unroll 4
-            for (uint32_t q = 0; q < a.pairs; ++q) {
+            for (uint32_t q = 0; q < p; ++q) {
                 const bool same = picks[q] == e;
-                own = same && all == 0 ? q : own;
-                n += same && q < p;
-                all += same;
+                own = same && n == 0 ? q : own;
+                n += same;
             }
         }
         owner[p] = (int16_t)own;
         before[p] = e >= 0 ? (int16_t)n : -1;
-        count[p] = (int16_t)all;
     }
     __syncthreads();
     if (threadIdx.x < 64) {
-        int items = 0, at = 0;
+        int items = 0;
         for (uint32_t p0 = 0; p0 < a.pairs; p0 += 64) {
             const uint32_t p = p0 + threadIdx.x;
             const bool fresh = p < a.pairs && before[p] == 0;
-            const int c = fresh ? count[p] : 0;
-            int sum = c;
-            for (int d = 1; d < 64; d <<= 1) {
-                const int o = __shfl_up(sum, d);
-                sum += (int)threadIdx.x >= d ? o : 0;
-            }
             const uint64_t all = __ballot(fresh);
             if (fresh) {
-                first[p] = (int16_t)(at + sum - c);
-                a.items[items + __builtin_popcountll(all & ((1ull << threadIdx.x) - 1))] = Q4Item{picks[p], at + sum - c, c, 0};
+                index[p] = (int16_t)(items + __builtin_popcountll(all & ((1ull << threadIdx.x) - 1)));
+                a.items[index[p]].expert = picks[p];
+                a.items[index[p]].count = 0;
             }
             items += __builtin_popcountll(all);
-            at += __shfl(sum, 63);
         }
         if (threadIdx.x == 0) *a.nitems = items;
     }
     __syncthreads();
     for (uint32_t p = threadIdx.x; p < a.pairs; p += THREADS)
-        if (before[p] >= 0) a.sorted[first[owner[p]] + before[p]] = (int32_t)p;
+        if (before[p] >= 0) {
+            Q4Item& it = a.items[index[owner[p]]];
+            it.pair[before[p]] = (int32_t)p;
+            atomicMax(&it.count, before[p] + 1);
+        }
 }
 
 __device__ __forceinline__ float swiglu(float g, float u) { return g / (1.0f + expf_path(0.0f - g)) * u; }
 
-// An activated value as TERMS bf16 numbers that add up to it (8 bits each).
-template <int TERMS>
-__device__ __forceinline__ void store_terms(uint16_t* h, size_t plane, size_t at, float v) {
-#pragma unroll
-    for (int i = 0; i < TERMS; ++i) {
+// An activated value as bf16 numbers that add up to it (8 bits each).
+__device__ __forceinline__ void store_terms(uint16_t* h, int terms, size_t plane, size_t at, float v) {
+    for (int i = 0; i < terms; ++i) {
         const uint16_t b = f2bf(v);
         h[(size_t)i * plane + at] = b;
         v = __builtin_fabsf(v) < __builtin_inff() ? v - bf2f(b) : 0.0f;
@@ -163,7 +172,7 @@ __device__ __forceinline__ void store_terms(uint16_t* h, size_t plane, size_t at
 // for the launches behind.
 enum Q4Rows { ONE_ROW, FEW_ROWS, ITEMS };
 
-template <bool BF, int GPC, int TERMS, int NT, int WK, int NB, int MODE>
+template <bool BF, bool SBF, int GPC, int NT, int WK, int NB, int MODE>
 __global__ void __launch_bounds__(64 * WK) q4_gateup_kernel(Q4MoeArgs a) {
     __shared__ f4v part[WK][NT][1][64];
     __shared__ int32_t picks[MODE == FEW_ROWS ? Q4_PAIRS : 16];
@@ -171,7 +180,7 @@ __global__ void __launch_bounds__(64 * WK) q4_gateup_kernel(Q4MoeArgs a) {
     const uint32_t u = blockIdx.y, chunks = q4_chunks(a.dims), tiles = (a.width + 7) / 8, r = lane & 15;
     int32_t e;
     const uint16_t* row[1] = {nullptr};
-    Q4Item it{};
+    int count = 0;
     if constexpr (MODE == ONE_ROW) {  // every slot by itself: nothing is compared before the weights are read
         e = a.pick[u];
         if ((uint32_t)e >= a.experts) return;
@@ -192,20 +201,21 @@ __global__ void __launch_bounds__(64 * WK) q4_gateup_kernel(Q4MoeArgs a) {
             for (uint32_t k = 0; k < a.slots; ++k)
                 if (picks[r * a.slots + k] == e) row[0] = a.x + (size_t)r * a.x_stride;
     } else {
-        if ((int)u >= *a.nitems) return;
-        it = a.items[u];
+        const Q4Item& it = a.items[u];
+        const int n = *a.nitems, p = it.pair[r];  // read together; what lies behind the items is not used
         e = it.expert;
-        const int32_t p = a.sorted[it.first + min((int)r, it.count - 1)];
+        count = it.count;
+        if ((int)u >= n) return;
         if (threadIdx.x < 16) picks[r] = p;
-        if ((int)r < it.count) row[0] = a.x + (size_t)((uint32_t)p / a.slots) * a.x_stride;
+        if ((int)r < count) row[0] = a.x + (size_t)((uint32_t)p / a.slots) * a.x_stride;
     }
     const uint32_t tile0 = min(blockIdx.x * NT, tiles - NT);  // the last block's tiles overlap
     const size_t tile_bytes = (size_t)chunks * q4_chunk_bytes(GPC);
     f4v out[NT][1];
 #pragma unroll
     for (int t = 0; t < NT; ++t) out[t][0] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
-    q4_stream<BF, GPC, 1, NT, NB, true>(a.gu + (size_t)e * a.gu_bytes + tile0 * tile_bytes, tile_bytes, wave, WK, chunks, row,
-                                        a.dims, lane, a.sbf, out);
+    q4_stream<BF, SBF, GPC, 1, NT, NB, true>(a.gu + (size_t)e * a.gu_bytes + tile0 * tile_bytes, tile_bytes, wave, WK, chunks, row,
+                                        a.dims, lane, out);
 #pragma unroll
     for (int t = 0; t < NT; ++t) part[wave][t][0][lane] = out[t][0];
     __syncthreads();
@@ -223,18 +233,18 @@ __global__ void __launch_bounds__(64 * WK) q4_gateup_kernel(Q4MoeArgs a) {
         }
         if constexpr (MODE == ITEMS) {
             p = picks[m];
-            is = is && m < it.count;
+            is = is && m < count;
         }
         if (!is) continue;
         const float v = swiglu(q4_total<WK, NT, 1>(part, t, 0, m, n), q4_total<WK, NT, 1>(part, t, 0, m, n + 8));
-        store_terms<TERMS>(a.h, (size_t)a.pairs * a.width, (size_t)p * a.width + col, v);
+        store_terms(a.h, a.terms, (size_t)a.pairs * a.width, (size_t)p * a.width + col, v);
     }
 }
 
 // ---- down -----------------------------------------------------------------------------------------------------------
 // One row: NT tiles of the output a block; its waves take the (slot, chunk) units in turn, weigh their sums in registers, and
 // terms (rows 0 .. TERMS - 1 of the instruction) and waves are added at the end.
-template <int GPC, int TERMS, int NT, int WK, int NB>
+template <bool SBF, int GPC, int TERMS, int NT, int WK, int NB>
 __global__ void __launch_bounds__(64 * WK) q4_down_one_kernel(Q4MoeArgs a) {
     __shared__ f4v part[WK][NT][1][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), term = lane & 15;
@@ -284,7 +294,7 @@ __global__ void __launch_bounds__(64 * WK) q4_down_one_kernel(Q4MoeArgs a) {
             f4v y[NT][1];
 #pragma unroll
             for (int t = 0; t < NT; ++t) y[t][0] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
-            q4_chunk<true, GPC, 1, NT>(words[i], par[i], x[i], a.sbf, y);
+            q4_chunk<true, SBF, GPC, 1, NT>(words[i], par[i], x[i], y);
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -310,37 +320,45 @@ __global__ void __launch_bounds__(64 * WK) q4_down_one_kernel(Q4MoeArgs a) {
 // Terms are rows of their own: rows 4 q .. 4 q + 3 of the instruction are quad q of the accumulators' lanes; with three
 // terms quad q holds term q of four pairs, with two quads 2 q and 2 q + 1 term q of eight, and adding lanes 16 (and 32)
 // apart adds the terms.
-template <int GPC, int TERMS, int NT, int WK, int NB>
+template <bool SBF, int GPC, int TERMS, int NT, int WK, int NB>
 __global__ void __launch_bounds__(64 * WK) q4_down_kernel(Q4MoeArgs a) {
     constexpr int PER = TERMS == 1 ? 16 : TERMS == 2 ? 8 : 4;  // pairs a product
-    if ((int)blockIdx.y >= *a.nitems) return;
-    const Q4Item it = a.items[blockIdx.y];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t chunks = q4_chunks(a.width), tiles = q4_tiles(a.dims), mine = (blockIdx.x * WK + wave) * NT;
-    if (mine >= tiles) return;
-    const uint32_t tile0 = min(mine, tiles - NT);  // the last wave's tiles overlap
+    const Q4Item& it = a.items[blockIdx.y];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quad = lane >> 4;
+    const int n = *a.nitems, e = it.expert, count = it.count;
+    const int from = it.pair[lane & (PER - 1)];
+    if ((int)blockIdx.y >= n) return;
+    const uint32_t chunks = q4_chunks(a.width), tiles = q4_tiles(a.dims);
     const size_t tile_bytes = (size_t)chunks * q4_chunk_bytes(GPC), plane = (size_t)a.pairs * a.width;
-    const uint8_t* w = a.down + (size_t)it.expert * a.down_bytes + tile0 * tile_bytes;
-    for (int m0 = 0; m0 < it.count; m0 += PER) {
-        const int m = m0 + (lane & (PER - 1)), term = (lane & 15) / PER;
+    const uint8_t* w = a.down + (size_t)e * a.down_bytes;
+    const int term = (lane & 15) / PER;
+    for (int m0 = 0; m0 < count; m0 += PER) {
         const uint16_t* row[1] = {nullptr};
-        if (m < it.count && term < TERMS) row[0] = a.h + term * plane + (size_t)a.sorted[it.first + m] * a.width;
-        f4v out[NT][1];
+        if (m0 + (lane & (PER - 1)) < count && term < TERMS)
+            row[0] = a.h + term * plane + (size_t)(m0 ? it.pair[m0 + (lane & (PER - 1))] : from) * a.width;
+        // the pairs of this lane's sums: value i is pair 4 (quad mod PER / 4) + i
+        const int at0 = m0 + 4 * (quad & (PER / 4 - 1));
+        int to[4];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) out[t][0] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
-        q4_stream<true, GPC, 1, NT, NB, true>(w, tile_bytes, 0, 1, chunks, row, a.width, lane, a.sbf, out);
+        for (int i = 0; i < 4; ++i) to[i] = it.pair[at0 + i];
+        const uint32_t mine = (blockIdx.x * WK + wave) * NT;
+        if (mine < tiles) {
+            const uint32_t tile0 = min(mine, tiles - NT);  // the last wave's tiles overlap
+            f4v out[NT][1];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int q = lane >> 4, at = m0 + 4 * (q & (PER / 4 - 1)) + i;  // the pair of this quad's value i
+            for (int t = 0; t < NT; ++t) out[t][0] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+            q4_stream<true, SBF, GPC, 1, NT, NB, true>(w + tile0 * tile_bytes, tile_bytes, 0, 1, chunks, row, a.width, lane,
+                                                  out);
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                float v = out[t][0][i];
-                if constexpr (TERMS == 3) v = v + lane_xor<16>(v);
-                if constexpr (TERMS >= 2) v = v + lane_xor<32>(v);
-                const uint32_t col = (tile0 + t) * 16 + (lane & 15);
-                if (at < it.count && q < PER / 4 && col < a.dims)
-                    a.y[(size_t)a.sorted[it.first + at] * a.dims + col] = v;
-            }
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    float v = out[t][0][i];
+                    if constexpr (TERMS == 3) v = v + lane_xor<16>(v);
+                    if constexpr (TERMS >= 2) v = v + lane_xor<32>(v);
+                    const uint32_t col = (tile0 + t) * 16 + (lane & 15);
+                    if (at0 + i < count && quad < PER / 4 && col < a.dims) a.y[(size_t)to[i] * a.dims + col] = v;
+                }
         }
     }
 }
@@ -349,7 +367,7 @@ __global__ void __launch_bounds__(64 * WK) q4_down_kernel(Q4MoeArgs a) {
 __global__ void __launch_bounds__(256) q4_combine_kernel(Q4MoeArgs a) {
     __shared__ int32_t pick[32];
     __shared__ float weight[32];
-    const uint32_t r = blockIdx.x, d = blockIdx.y * 256 + threadIdx.x;
+    const uint32_t r = blockIdx.x, d = (blockIdx.y * 256 + threadIdx.x) * 4;
     if (threadIdx.x < a.slots) pick[threadIdx.x] = a.pick[(size_t)r * a.slots + threadIdx.x];
     __syncthreads();
     if (threadIdx.x < a.slots) {  // an expert named again adds its weight to the first naming
@@ -366,45 +384,62 @@ __global__ void __launch_bounds__(256) q4_combine_kernel(Q4MoeArgs a) {
     }
     __syncthreads();
     if (d >= a.dims) return;
-    float v = 0.0f;
-    for (uint32_t k = 0; k < a.slots; ++k)
-        if (pick[k] >= 0) v = __builtin_fmaf(weight[k], a.y[((size_t)r * a.slots + k) * a.dims + d], v);
-    store_act(a.out, a.out_dtype, (size_t)r * a.dims + d, v);
+    f4v v{0.0f, 0.0f, 0.0f, 0.0f};
+    const float* y = a.y + (size_t)r * a.slots * a.dims + d;
+    for (uint32_t k0 = 0; k0 < a.slots; k0 += 8) {  // eight slots' loads at once; what is no expert's is not used
+        f4v p[8];
+        bool has[8];
+#pragma unroll
+        for (uint32_t k = 0; k < 8; ++k) {
+            has[k] = k0 + k < a.slots && pick[k0 + k] >= 0;
+            p[k] = *reinterpret_cast<const f4v*>(y + (size_t)min(k0 + k, a.slots - 1) * a.dims);
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < 8; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = has[k] ? __builtin_fmaf(weight[k0 + k], p[k][i], v[i]) : v[i];
+    }
+    const size_t at = (size_t)r * a.dims + d;
+    if (a.out_dtype == F32) {
+        typedef f4v f4v_a4 __attribute__((aligned(4)));
+        *reinterpret_cast<f4v_a4*>(static_cast<float*>(a.out) + at) = v;
+    } else {
+        typedef u2v u2v_a2 __attribute__((aligned(2)));
+        uint16_t b[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) b[i] = a.out_dtype == BF16 ? f2bf(v[i]) : f2h(v[i]);
+        *reinterpret_cast<u2v_a2*>(static_cast<uint16_t*>(a.out) + at) =
+            u2v{(uint32_t)b[0] | (uint32_t)b[1] << 16, (uint32_t)b[2] | (uint32_t)b[3] << 16};
+    }
 }
 
 // ---- launches -------------------------------------------------------------------------------------------------------
-template <int GPC, int TERMS>
-static void launch_moe(hipStream_t s, const Q4MoeArgs& a, bool bf, uint32_t max_items) {
-    const uint32_t tiles = (a.width + 7) / 8, dtiles = q4_tiles(a.dims);
-    auto gateup = [&](auto bf_, auto nt_, auto mode_, uint32_t blocks) {
-        constexpr int NT = decltype(nt_)::value, WK = 8;
-        q4_gateup_kernel<decltype(bf_)::value, GPC, TERMS, NT, WK, 3, decltype(mode_)::value>
-            <<<dim3((tiles + NT - 1) / NT, blocks), 64 * WK, 0, s>>>(a);
-    };
-    auto with = [&](auto nt_, auto mode_, uint32_t blocks) {
-        if (bf) gateup(std::true_type{}, nt_, mode_, blocks);
-        else gateup(std::false_type{}, nt_, mode_, blocks);
-    };
-    using One = std::integral_constant<int, 1>;
-    using Two = std::integral_constant<int, 2>;
-    if (a.rows == 1) {
-        with(One{}, std::integral_constant<int, ONE_ROW>{}, a.pairs);
-        q4_down_one_kernel<GPC, TERMS, 1, 8, 2><<<dtiles, 512, 0, s>>>(a);
-        return;
-    }
-    if (a.rows <= Q4_ROWS) {
-        const std::integral_constant<int, FEW_ROWS> few{};
-        if (a.rows <= 4 || tiles < 2) with(One{}, few, a.pairs + 1);
-        else with(Two{}, few, a.pairs + 1);
-    } else {
-        q4_group_kernel<<<1, 1024, 0, s>>>(a);
-        const std::integral_constant<int, ITEMS> items{};
-        if (tiles < 2) with(One{}, items, max_items);
-        else with(Two{}, items, max_items);
-    }
-    if (dtiles >= 4) q4_down_kernel<GPC, TERMS, 4, 4, 2><<<dim3((dtiles + 15) / 16, max_items), 256, 0, s>>>(a);
-    else q4_down_kernel<GPC, TERMS, 1, 4, 2><<<dim3((dtiles + 3) / 4, max_items), 256, 0, s>>>(a);
-    q4_combine_kernel<<<dim3(a.rows, (a.dims + 255) / 256), 256, 0, s>>>(a);
+static void launch_gateup(hipStream_t s, const Q4MoeArgs& a, bool bf, bool sbf, int gpc, uint32_t max_items) {
+    const uint32_t tiles = (a.width + 7) / 8;
+    q4_types(bf, sbf, gpc, [&](auto gpc_, auto bf_, auto sbf_) {
+        constexpr bool BF = decltype(bf_)::value, SBF = decltype(sbf_)::value;
+        constexpr int GPC = decltype(gpc_)::value;
+        const dim3 one(tiles, a.pairs + (a.rows > 1)), two((tiles + 1) / 2, a.pairs + 1);
+        if (a.rows == 1) q4_gateup_kernel<BF, SBF, GPC, 1, 8, 3, ONE_ROW><<<one, 512, 0, s>>>(a);
+        else if (a.rows <= 4 || (a.rows <= Q4_ROWS && tiles < 2)) q4_gateup_kernel<BF, SBF, GPC, 1, 8, 3, FEW_ROWS><<<one, 512, 0, s>>>(a);
+        else if (a.rows <= Q4_ROWS) q4_gateup_kernel<BF, SBF, GPC, 2, 8, 3, FEW_ROWS><<<two, 512, 0, s>>>(a);
+        else if (tiles < 2) q4_gateup_kernel<BF, SBF, GPC, 1, 8, 3, ITEMS><<<dim3(1, max_items), 512, 0, s>>>(a);
+        else q4_gateup_kernel<BF, SBF, GPC, 2, 8, 3, ITEMS><<<dim3((tiles + 1) / 2, max_items), 512, 0, s>>>(a);
+    });
+}
+
+template <int TERMS>
+static void launch_down(hipStream_t s, const Q4MoeArgs& a, bool sbf, int gpc, uint32_t max_items) {
+    const uint32_t tiles = q4_tiles(a.dims);
+    q4_types(true, sbf, gpc, [&](auto gpc_, auto bf_, auto sbf_) {
+        if constexpr (decltype(bf_)::value) {
+            constexpr bool SBF = decltype(sbf_)::value;
+            constexpr int GPC = decltype(gpc_)::value;
+            if (a.rows == 1) q4_down_one_kernel<SBF, GPC, TERMS, 1, 8, 2><<<tiles, 512, 0, s>>>(a);
+            else if (tiles >= 4) q4_down_kernel<SBF, GPC, TERMS, 4, 8, 1><<<dim3((tiles + 31) / 32, max_items), 512, 0, s>>>(a);
+            else q4_down_kernel<SBF, GPC, TERMS, 1, 4, 1><<<dim3((tiles + 3) / 4, max_items), 256, 0, s>>>(a);
+        }
+    });
 }
 
 // Terms of the activated values: what the output's type can show (bf16 8 bits, fp16 11, fp32 24).
@@ -435,11 +470,10 @@ static size_t q4_carve(ea_q4_scratch* s, uint64_t base, const ea_q4_experts* ex,
         at += up256(bytes);
         return p;
     };
-    s->sorted = take(4 * pairs);
     s->items = take(sizeof(Q4Item) * q4_max_items(ex->count, pairs));
     s->count = take(4);
     s->h = take(3 * 2 * pairs * ex->width);
-    s->y = take(4 * pairs * ex->dims);
+    s->y = take(4 * (size_t)pairs * ex->dims);
     s->rows = rows;
     s->slots = slots;
     return at;
@@ -484,7 +518,7 @@ int ea_q4_routed(ea_stream_t stream, const void* x, int x_dtype, uint32_t x_stri
     EA_REQUIRE_CTX(ctx_);
     (void)ctx_;
     if (R == 0) return EA_OK;
-    const int gpc = 128 / (int)ex->group, terms = q4_terms(out_dtype);
+    const int gpc = 128 / (int)ex->group;
     Q4MoeArgs a{};
     a.x = static_cast<const uint16_t*>(x);
     a.x_stride = x_stride;
@@ -494,7 +528,6 @@ int ea_q4_routed(ea_stream_t stream, const void* x, int x_dtype, uint32_t x_stri
     a.down = dptr<const uint8_t>(ex->down);
     a.gu_bytes = (size_t)((ex->width + 7) / 8) * q4_chunks(ex->dims) * q4_chunk_bytes(gpc);
     a.down_bytes = (size_t)q4_tiles(ex->dims) * q4_chunks(ex->width) * q4_chunk_bytes(gpc);
-    a.sorted = dptr<int32_t>(sc->sorted);
     a.nitems = dptr<int32_t>(sc->count);
     a.items = dptr<Q4Item>(sc->items);
     a.h = dptr<uint16_t>(sc->h);
@@ -507,18 +540,16 @@ int ea_q4_routed(ea_stream_t stream, const void* x, int x_dtype, uint32_t x_stri
     a.experts = ex->count;
     a.slots = sc->slots;
     a.out_dtype = out_dtype;
-    a.sbf = ex->s_dtype == BF16;
+    a.terms = q4_terms(out_dtype);
     const uint32_t max_items = q4_max_items(a.experts, a.pairs);
     hipStream_t s = as_stream(stream);
-    auto go = [&](auto gpc_) {
-        constexpr int GPC = decltype(gpc_)::value;
-        if (terms == 1) launch_moe<GPC, 1>(s, a, x_dtype == BF16, max_items);
-        else if (terms == 2) launch_moe<GPC, 2>(s, a, x_dtype == BF16, max_items);
-        else launch_moe<GPC, 3>(s, a, x_dtype == BF16, max_items);
-    };
-    if (gpc == 4) go(std::integral_constant<int, 4>{});
-    else if (gpc == 2) go(std::integral_constant<int, 2>{});
-    else go(std::integral_constant<int, 1>{});
+    const bool sbf = ex->s_dtype == BF16;
+    if (R > Q4_ROWS) q4_group_kernel<<<1, 1024, 0, s>>>(a);
+    launch_gateup(s, a, x_dtype == BF16, sbf, gpc, max_items);
+    if (a.terms == 1) launch_down<1>(s, a, sbf, gpc, max_items);
+    else if (a.terms == 2) launch_down<2>(s, a, sbf, gpc, max_items);
+    else launch_down<3>(s, a, sbf, gpc, max_items);
+    if (R > 1) q4_combine_kernel<<<dim3(R, (a.dims + 1023) / 1024), 256, 0, s>>>(a);
     return launched();
 }
 
