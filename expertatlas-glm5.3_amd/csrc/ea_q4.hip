@@ -5,7 +5,7 @@
 #include <type_traits>
 
 #include "ea_host.hpp"
-#include "ea_q4.hpp"
+#include "ea_q4_gemm.hpp"
 
 namespace ea {
 
@@ -106,6 +106,29 @@ __global__ void __launch_bounds__(64 * WK) q4_linear_kernel(Q4LinArgs a) {
     }
 }
 
+// More rows: 16 MT rows and 4 NT tiles a block.
+template <bool BF, bool SBF, int GPC, int MT, int NT>
+__global__ void __launch_bounds__(Q4_GEMM_THREADS, 2) q4_linear_gemm_kernel(Q4LinArgs a) {
+    __shared__ __attribute__((aligned(16))) uint8_t lds[q4_gemm_lds<MT>()];
+    const Q4Job job = a.job[blockIdx.z];
+    const uint32_t tiles = q4_tiles(job.n), m0 = blockIdx.y * 16 * MT;
+    if (blockIdx.x * 4 * NT >= tiles) return;
+    const int lane = threadIdx.x & 63;
+    q4_gemm<BF, SBF, GPC, MT, NT>(
+        lds, job.w, tiles, a.k, 1, 0, blockIdx.x, 1u << 24,
+        [&](uint32_t i) { return a.x + (size_t)min(m0 + i, a.m - 1) * a.x_stride; },
+        [&](uint32_t tile, const f4v(&v)[MT]) {
+            const uint32_t n = tile * 16 + (lane & 15);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t r = m0 + 16 * mt + 4 * (lane >> 4) + i;
+                    if (r < a.m && n < job.n) store_act(job.y, job.y_dtype, (size_t)r * job.n + n, v[mt][i]);
+                }
+        });
+}
+
 static int launch_linear(hipStream_t s, const Q4LinArgs& a, uint32_t tiles, bool bf, bool sbf, int gpc) {
     auto go = [&](auto gpc_, auto bf_, auto sbf_) {
         constexpr int GPC = decltype(gpc_)::value;
@@ -114,7 +137,13 @@ static int launch_linear(hipStream_t s, const Q4LinArgs& a, uint32_t tiles, bool
         if (a.m <= 16) {
             if (tiles * jobs < 512) q4_linear_kernel<BF, SBF, GPC, 1, 1, 16, 3><<<dim3(tiles, 1, jobs), 1024, 0, s>>>(a);
             else q4_linear_kernel<BF, SBF, GPC, 1, 2, 8, 3><<<dim3((tiles + 1) / 2, 1, jobs), 512, 0, s>>>(a);
-        } else q4_linear_kernel<BF, SBF, GPC, 4, 1, 8, 1><<<dim3(tiles, (a.m + 63) / 64, jobs), 512, 0, s>>>(a);
+        } else {
+#ifndef LV
+#define LV 2
+#endif
+            if (LV == 0) q4_linear_kernel<BF, SBF, GPC, 4, 1, 8, 1><<<dim3(tiles, (a.m + 63) / 64, jobs), 512, 0, s>>>(a);
+            else q4_linear_gemm_kernel<BF, SBF, GPC, 4, LV ? LV : 1><<<dim3((tiles + 4 * LV - 1) / (4 * (LV ? LV : 1)), (a.m + 63) / 64, jobs), Q4_GEMM_THREADS, 0, s>>>(a);
+        }
     };
     q4_types(bf, sbf, gpc, go);
     return launched();

@@ -10,18 +10,18 @@
 #include <type_traits>
 
 #include "ea_host.hpp"
-#include "ea_q4.hpp"
+#include "ea_q4_gemm.hpp"
 
 namespace ea {
 
 constexpr uint32_t Q4_MAX_EXPERTS = 4096;
-constexpr uint32_t Q4_ITEM = 16;                       // rows an item
+constexpr uint32_t Q4_ITEM = 16, Q4_BIG_ITEM = 64;         // pairs an item
 constexpr uint32_t Q4_ROWS = 16, Q4_PAIRS = Q4_ROWS * 32;  // rows and pairs that are grouped beside the first products
 
-// An expert and up to 16 of its pairs (row * slots + slot).
+// An expert and up to Q4_ITEM or Q4_BIG_ITEM of its pairs (row * slots + slot).
 struct Q4Item {
     int32_t expert, count;
-    int32_t pair[Q4_ITEM];
+    int32_t pair[Q4_BIG_ITEM];
 };
 
 struct Q4MoeArgs {
@@ -36,7 +36,7 @@ struct Q4MoeArgs {
     uint16_t* h;                  // bf16 [terms][pairs][width]
     float* y;                     // fp32 [pairs][dims]
     void* out;
-    uint32_t rows, pairs, dims, width, experts, slots;
+    uint32_t rows, pairs, dims, width, experts, slots, item;  // item: pairs an item at most
     int out_dtype, terms;
 };
 
@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(1024) q4_group_kernel(Q4MoeArgs a) {
     __syncthreads();
     uint32_t base = 0;
     for (uint32_t e0 = 0; e0 < a.experts; e0 += 1024) {  // an exclusive scan of the experts' items, 1024 experts a step
-        const uint32_t e = e0 + t, c = e < a.experts ? count[e] : 0, n = (c + Q4_ITEM - 1) / Q4_ITEM;
+        const uint32_t e = e0 + t, c = e < a.experts ? count[e] : 0, n = (c + a.item - 1) / a.item;
         uint32_t v = n;
         for (int d = 1; d < 64; d <<= 1) {
             const uint32_t o = __shfl_up(v, d);
@@ -81,14 +81,14 @@ __global__ void __launch_bounds__(1024) q4_group_kernel(Q4MoeArgs a) {
         }
         for (uint32_t i = 0; i < n; ++i) {
             a.items[item + i].expert = (int32_t)e;
-            a.items[item + i].count = (int32_t)min(c - i * Q4_ITEM, Q4_ITEM);
+            a.items[item + i].count = (int32_t)min(c - i * a.item, a.item);
         }
         __syncthreads();
     }
     if (t == 0) *a.nitems = (int32_t)base;
     const auto place = [&](uint32_t p, uint32_t e) {
         const uint32_t at = atomicAdd(&count[e], 1u);
-        a.items[start[e] + at / Q4_ITEM].pair[at % Q4_ITEM] = (int32_t)p;
+        a.items[start[e] + at / a.item].pair[at % a.item] = (int32_t)p;
     };
 #pragma unroll
     for (int i = 0; i < KEEP; ++i)
@@ -363,6 +363,62 @@ __global__ void __launch_bounds__(64 * WK) q4_down_kernel(Q4MoeArgs a) {
     }
 }
 
+// ---- long items -----------------------------------------------------------------------------------------------------
+// An item's products by q4_gemm, with as many row groups as it has.
+template <bool BF, bool SBF, int GPC, int NT, typename ROW, typename STORE>
+__device__ __forceinline__ void q4_item_gemm(uint8_t* lds, int count, const uint8_t* w, uint32_t tiles, uint32_t k,
+                                             uint32_t terms, size_t plane, uint32_t cb, uint32_t cb_step, ROW row,
+                                             STORE store) {
+    if (count <= 16) q4_gemm<BF, SBF, GPC, 1, NT>(lds, w, tiles, k, terms, plane, cb, cb_step, row, store);
+    else if (count <= 32) q4_gemm<BF, SBF, GPC, 2, NT>(lds, w, tiles, k, terms, plane, cb, cb_step, row, store);
+    else q4_gemm<BF, SBF, GPC, 4, NT>(lds, w, tiles, k, terms, plane, cb, cb_step, row, store);
+}
+
+template <bool BF, bool SBF, int GPC, int NT>
+__global__ void __launch_bounds__(Q4_GEMM_THREADS, 2) q4_gateup_gemm_kernel(Q4MoeArgs a) {
+    __shared__ __attribute__((aligned(16))) uint8_t lds[q4_gemm_lds<4>()];
+    const Q4Item& it = a.items[blockIdx.y];
+    const int n = *a.nitems, e = it.expert, count = it.count, lane = threadIdx.x & 63;
+    if ((int)blockIdx.y >= n) return;
+    q4_item_gemm<BF, SBF, GPC, NT>(
+        lds, count, a.gu + (size_t)e * a.gu_bytes, (a.width + 7) / 8, a.dims, 1, 0, blockIdx.x, 1u << 24,
+        [&](int i) { return a.x + (size_t)((uint32_t)it.pair[min(i, count - 1)] / a.slots) * a.x_stride; },
+        [&](uint32_t tile, const auto& v) {
+            const uint32_t col = tile * 8 + (lane & 7);
+#pragma unroll
+            for (int mt = 0; mt < (int)(sizeof(v) / sizeof(f4v)); ++mt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float u = lane_xor<8>(v[mt][i]);  // lanes 0 .. 7 of 16 have the gate, the others the up column
+                    const int m = 16 * mt + 4 * (lane >> 4) + i;
+                    if ((lane & 8) || m >= count || col >= a.width) continue;
+                    store_terms(a.h, a.terms, (size_t)a.pairs * a.width, (size_t)it.pair[m] * a.width + col,
+                                swiglu(v[mt][i], u));
+                }
+        });
+}
+
+template <bool SBF, int GPC, int NT>
+__global__ void __launch_bounds__(Q4_GEMM_THREADS, 2) q4_down_gemm_kernel(Q4MoeArgs a) {
+    __shared__ __attribute__((aligned(16))) uint8_t lds[q4_gemm_lds<4>()];
+    const Q4Item& it = a.items[blockIdx.y];
+    const int n = *a.nitems, e = it.expert, count = it.count, lane = threadIdx.x & 63;
+    if ((int)blockIdx.y >= n) return;
+    q4_item_gemm<true, SBF, GPC, NT>(
+        lds, count, a.down + (size_t)e * a.down_bytes, q4_tiles(a.dims), a.width, a.terms, (size_t)a.pairs * a.width,
+        blockIdx.x, gridDim.x, [&](int i) { return a.h + (size_t)it.pair[min(i, count - 1)] * a.width; },
+        [&](uint32_t tile, const auto& v) {
+            const uint32_t col = tile * 16 + (lane & 15);
+#pragma unroll
+            for (int mt = 0; mt < (int)(sizeof(v) / sizeof(f4v)); ++mt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int m = 16 * mt + 4 * (lane >> 4) + i;
+                    if (m < count && col < a.dims) a.y[(size_t)it.pair[m] * a.dims + col] = v[mt][i];
+                }
+        });
+}
+
 // ---- a row's slots, in order ----------------------------------------------------------------------------------------
 __global__ void __launch_bounds__(256) q4_combine_kernel(Q4MoeArgs a) {
     __shared__ int32_t pick[32];
@@ -423,6 +479,13 @@ static void launch_gateup(hipStream_t s, const Q4MoeArgs& a, bool bf, bool sbf, 
         if (a.rows == 1) q4_gateup_kernel<BF, SBF, GPC, 1, 8, 3, ONE_ROW><<<one, 512, 0, s>>>(a);
         else if (a.rows <= 4 || (a.rows <= Q4_ROWS && tiles < 2)) q4_gateup_kernel<BF, SBF, GPC, 1, 8, 3, FEW_ROWS><<<one, 512, 0, s>>>(a);
         else if (a.rows <= Q4_ROWS) q4_gateup_kernel<BF, SBF, GPC, 2, 8, 3, FEW_ROWS><<<two, 512, 0, s>>>(a);
+#ifndef GNT
+#define GNT 4
+#define DNT2 4
+#define DSP 6
+#endif
+        else if (a.item == Q4_BIG_ITEM)
+            q4_gateup_gemm_kernel<BF, SBF, GPC, GNT><<<dim3((tiles + 4 * GNT - 1) / (4 * GNT), max_items), Q4_GEMM_THREADS, 0, s>>>(a);
         else if (tiles < 2) q4_gateup_kernel<BF, SBF, GPC, 1, 8, 3, ITEMS><<<dim3(1, max_items), 512, 0, s>>>(a);
         else q4_gateup_kernel<BF, SBF, GPC, 2, 8, 3, ITEMS><<<dim3((tiles + 1) / 2, max_items), 512, 0, s>>>(a);
     });
@@ -436,6 +499,8 @@ static void launch_down(hipStream_t s, const Q4MoeArgs& a, bool sbf, int gpc, ui
             constexpr bool SBF = decltype(sbf_)::value;
             constexpr int GPC = decltype(gpc_)::value;
             if (a.rows == 1) q4_down_one_kernel<SBF, GPC, TERMS, 1, 8, 2><<<tiles, 512, 0, s>>>(a);
+            else if (a.item == Q4_BIG_ITEM)
+                q4_down_gemm_kernel<SBF, GPC, DNT2><<<dim3(std::min((tiles + 4 * DNT2 - 1) / (4 * DNT2), (uint32_t)DSP), max_items), Q4_GEMM_THREADS, 0, s>>>(a);
             else if (tiles >= 4) q4_down_kernel<SBF, GPC, TERMS, 4, 8, 1><<<dim3((tiles + 31) / 32, max_items), 512, 0, s>>>(a);
             else q4_down_kernel<SBF, GPC, TERMS, 1, 4, 1><<<dim3((tiles + 3) / 4, max_items), 256, 0, s>>>(a);
         }
@@ -445,8 +510,8 @@ static void launch_down(hipStream_t s, const Q4MoeArgs& a, bool sbf, int gpc, ui
 // Terms of the activated values: what the output's type can show (bf16 8 bits, fp16 11, fp32 24).
 static int q4_terms(int out_dtype) { return out_dtype == BF16 ? 1 : out_dtype == F16 ? 2 : 3; }
 
-static uint32_t q4_max_items(uint32_t experts, size_t pairs) {
-    const size_t full = pairs / Q4_ITEM, some = pairs < experts ? pairs : experts;
+static uint32_t q4_max_items(uint32_t experts, size_t pairs, uint32_t item = Q4_ITEM) {
+    const size_t full = pairs / item, some = pairs < experts ? pairs : experts;
     return (uint32_t)(full + some);
 }
 
@@ -541,7 +606,11 @@ int ea_q4_routed(ea_stream_t stream, const void* x, int x_dtype, uint32_t x_stri
     a.slots = sc->slots;
     a.out_dtype = out_dtype;
     a.terms = q4_terms(out_dtype);
-    const uint32_t max_items = q4_max_items(a.experts, a.pairs);
+    #ifndef BIGR
+#define BIGR 128
+#endif
+    a.item = R > BIGR ? Q4_BIG_ITEM : Q4_ITEM;
+    const uint32_t max_items = q4_max_items(a.experts, a.pairs, a.item);
     hipStream_t s = as_stream(stream);
     const bool sbf = ex->s_dtype == BF16;
     if (R > Q4_ROWS) q4_group_kernel<<<1, 1024, 0, s>>>(a);
