@@ -114,9 +114,9 @@ __global__ void __launch_bounds__(Q4_GEMM_THREADS, 2) q4_linear_gemm_kernel(Q4Li
     const uint32_t tiles = q4_tiles(job.n), m0 = blockIdx.y * 16 * MT;
     if (blockIdx.x * 4 * NT >= tiles) return;
     const int lane = threadIdx.x & 63;
-    q4_gemm<BF, SBF, GPC, MT, NT>(
+    q4_gemm<BF, SBF, GPC, MT, NT, true, false>(
         lds, job.w, tiles, a.k, 1, 0, blockIdx.x, 1u << 24,
-        [&](uint32_t i) { return a.x + (size_t)min(m0 + i, a.m - 1) * a.x_stride; },
+        [&](uint32_t i) { return a.x + (size_t)min(m0 + i, a.m - 1) * a.x_stride; }, nullptr,
         [&](uint32_t tile, const f4v(&v)[MT]) {
             const uint32_t n = tile * 16 + (lane & 15);
 #pragma unroll

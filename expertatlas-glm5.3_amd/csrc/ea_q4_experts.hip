@@ -31,26 +31,32 @@ struct Q4MoeArgs {
     const float* wts;
     const uint8_t *gu, *down;
     size_t gu_bytes, down_bytes;  // one expert's
-    int32_t* nitems;
+    int32_t* nitems;              // items, full ones among them
     Q4Item* items;
     uint16_t* h;                  // bf16 [terms][pairs][width]
+    uint8_t *xsums, *hsums;       // sums over groups of a row of x, of a pair of h (q4_row_sums)
     float* y;                     // fp32 [pairs][dims]
     void* out;
     uint32_t rows, pairs, dims, width, experts, slots, item;  // item: pairs an item at most
     int out_dtype, terms;
+    uint32_t group;
+    bool bf;
 };
 
 // ---- grouping -----------------------------------------------------------------------------------------------------
 // One block: the pairs of each expert counted, the items before each expert scanned, the pairs placed (in any order within an
-// expert). A pick outside 0 .. experts - 1 is a slot without an expert.
-__global__ void __launch_bounds__(1024) q4_group_kernel(Q4MoeArgs a) {
-    __shared__ uint32_t count[Q4_MAX_EXPERTS], start[Q4_MAX_EXPERTS], sums[16];
+// expert). Full items come before all others, so that the longest work starts first. A pick outside 0 .. experts - 1 is a slot
+// without an expert.
+__device__ void q4_group(const Q4MoeArgs& a) {
+    __shared__ uint32_t count[Q4_MAX_EXPERTS], full[Q4_MAX_EXPERTS], rest[Q4_MAX_EXPERTS], sums[2][16], all;
+    __shared__ uint16_t nfull[Q4_MAX_EXPERTS];  // at most EA_Q4_MAX_PAIRS / Q4_ITEM
     constexpr int KEEP = 8;  // picks a thread keeps between the passes
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     uint32_t kept[KEEP];
 #pragma unroll
     for (int i = 0; i < KEEP; ++i) kept[i] = (uint32_t)(t + 1024u * i) < a.pairs ? (uint32_t)a.pick[t + 1024 * i] : 0xffffffffu;
     for (uint32_t e = t; e < a.experts; e += 1024) count[e] = 0;
+    if (t == 0) all = 0;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < KEEP; ++i)
@@ -60,35 +66,49 @@ __global__ void __launch_bounds__(1024) q4_group_kernel(Q4MoeArgs a) {
         if (e < a.experts) atomicAdd(&count[e], 1u);
     }
     __syncthreads();
-    uint32_t base = 0;
-    for (uint32_t e0 = 0; e0 < a.experts; e0 += 1024) {  // an exclusive scan of the experts' items, 1024 experts a step
-        const uint32_t e = e0 + t, c = e < a.experts ? count[e] : 0, n = (c + a.item - 1) / a.item;
-        uint32_t v = n;
+    uint32_t mine = 0;
+    for (uint32_t e = t; e < a.experts; e += 1024) mine += count[e] / a.item;
+    if (mine) atomicAdd(&all, mine);
+    __syncthreads();
+    uint32_t fbase = 0, rbase = all;
+    for (uint32_t e0 = 0; e0 < a.experts; e0 += 1024) {  // exclusive scans, 1024 experts a step
+        const uint32_t e = e0 + t, c = e < a.experts ? count[e] : 0, n = c / a.item, r = c % a.item != 0;
+        uint32_t v = n, w = r;
         for (int d = 1; d < 64; d <<= 1) {
-            const uint32_t o = __shfl_up(v, d);
-            v += lane >= d ? o : 0;
+            const uint32_t ov = __shfl_up(v, d), ow = __shfl_up(w, d);
+            v += lane >= d ? ov : 0;
+            w += lane >= d ? ow : 0;
         }
-        if (lane == 63) sums[wave] = v;
+        if (lane == 63) sums[0][wave] = v, sums[1][wave] = w;
         __syncthreads();
-        uint32_t item = base + v - n;
+        uint32_t fi = fbase + v - n, ri = rbase + w - r;
         for (int i = 0; i < 16; ++i) {
-            item += i < wave ? sums[i] : 0;
-            base += sums[i];
+            fi += i < wave ? sums[0][i] : 0;
+            ri += i < wave ? sums[1][i] : 0;
+            fbase += sums[0][i];
+            rbase += sums[1][i];
         }
         if (e < a.experts) {
-            start[e] = item;
+            full[e] = fi;
+            rest[e] = ri;
+            nfull[e] = (uint16_t)n;
             count[e] = 0;
         }
         for (uint32_t i = 0; i < n; ++i) {
-            a.items[item + i].expert = (int32_t)e;
-            a.items[item + i].count = (int32_t)min(c - i * a.item, a.item);
+            a.items[fi + i].expert = (int32_t)e;
+            a.items[fi + i].count = (int32_t)a.item;
+        }
+        if (r) {
+            a.items[ri].expert = (int32_t)e;
+            a.items[ri].count = (int32_t)(c % a.item);
         }
         __syncthreads();
     }
-    if (t == 0) *a.nitems = (int32_t)base;
+    const uint32_t base = rbase;
+    if (t == 0) a.nitems[0] = (int32_t)base, a.nitems[1] = (int32_t)all;
     const auto place = [&](uint32_t p, uint32_t e) {
-        const uint32_t at = atomicAdd(&count[e], 1u);
-        a.items[start[e] + at / a.item].pair[at % a.item] = (int32_t)p;
+        const uint32_t at = atomicAdd(&count[e], 1u), i = at / a.item;
+        a.items[i < nfull[e] ? full[e] + i : rest[e]].pair[at % a.item] = (int32_t)p;
     };
 #pragma unroll
     for (int i = 0; i < KEEP; ++i)
@@ -97,6 +117,20 @@ __global__ void __launch_bounds__(1024) q4_group_kernel(Q4MoeArgs a) {
         const uint32_t e = (uint32_t)a.pick[p];
         if (e < a.experts) place(p, e);
     }
+}
+
+// The grouping, and with more blocks beside it the rows' sums over groups, a wave a row.
+__global__ void __launch_bounds__(1024) q4_group_kernel(Q4MoeArgs a) {
+    if (blockIdx.x == 0) {
+        q4_group(a);
+        return;
+    }
+    const uint32_t i = (blockIdx.x - 1) * 16 + (threadIdx.x >> 6);
+    if (i >= a.rows) return;
+    uint8_t* to = a.xsums + (size_t)i * q4_sum_bytes(a.dims / a.group);
+    const uint16_t* row = a.x + (size_t)i * a.x_stride;
+    if (a.bf) q4_row_sums<true>(row, 1, 0, a.dims, a.group, to, threadIdx.x & 63);
+    else q4_row_sums<false>(row, 1, 0, a.dims, a.group, to, threadIdx.x & 63);
 }
 
 // The same for up to 16 rows, in the order of the experts' first pairs, by a block beside the first products (picks: the
@@ -363,26 +397,55 @@ __global__ void __launch_bounds__(64 * WK) q4_down_kernel(Q4MoeArgs a) {
     }
 }
 
-// ---- long items -----------------------------------------------------------------------------------------------------
-// An item's products by q4_gemm, with as many row groups as it has.
-template <bool BF, bool SBF, int GPC, int NT, typename ROW, typename STORE>
-__device__ __forceinline__ void q4_item_gemm(uint8_t* lds, int count, const uint8_t* w, uint32_t tiles, uint32_t k,
-                                             uint32_t terms, size_t plane, uint32_t cb, uint32_t cb_step, ROW row,
-                                             STORE store) {
-    if (count <= 16) q4_gemm<BF, SBF, GPC, 1, NT>(lds, w, tiles, k, terms, plane, cb, cb_step, row, store);
-    else if (count <= 32) q4_gemm<BF, SBF, GPC, 2, NT>(lds, w, tiles, k, terms, plane, cb, cb_step, row, store);
-    else q4_gemm<BF, SBF, GPC, 4, NT>(lds, w, tiles, k, terms, plane, cb, cb_step, row, store);
+// ---- the sums over groups of the activated values, for the biases of long items -------------------------------------------
+__global__ void __launch_bounds__(256) q4_hsums_kernel(Q4MoeArgs a) {
+    const uint32_t i = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (i < a.pairs && (uint32_t)a.pick[i] < a.experts)
+        q4_row_sums<true>(a.h + (size_t)i * a.width, a.terms, (size_t)a.pairs * a.width, a.width, a.group,
+                          a.hsums + (size_t)i * q4_sum_bytes(a.width / a.group), threadIdx.x & 63);
 }
 
+// ---- long items -----------------------------------------------------------------------------------------------------
+// An item's products by q4_gemm, with as many row groups as it has.
+template <bool BF, bool SBF, int GPC, int NT, bool RESIDENT, typename ROW, typename SUMS, typename STORE>
+__device__ __forceinline__ void q4_item_gemm(uint8_t* lds, int count, const uint8_t* w, uint32_t tiles, uint32_t k,
+                                             uint32_t terms, size_t plane, uint32_t cb, uint32_t cb_step, ROW row,
+                                             SUMS sums, STORE store) {
+    if (count <= 16) q4_gemm<BF, SBF, GPC, 1, NT, false, RESIDENT>(lds, w, tiles, k, terms, plane, cb, cb_step, row, sums, store);
+    else if (count <= 32) q4_gemm<BF, SBF, GPC, 2, NT, false, RESIDENT>(lds, w, tiles, k, terms, plane, cb, cb_step, row, sums, store);
+    else q4_gemm<BF, SBF, GPC, 4, NT, false, RESIDENT>(lds, w, tiles, k, terms, plane, cb, cb_step, row, sums, store);
+}
+
+// Blocks go to the card's eight dies in turn, and each die has an L2 of its own: die x takes the x-th eighth of the full items
+// (of the partial ones), a run by expert, and all column blocks of its items, so that an expert's weights and an item's rows
+// come from memory once a die.
+struct Q4Place {
+    int item;  // -1: none
+    uint32_t cb;
+};
+constexpr int Q4_DIES = 8;
+__device__ __forceinline__ Q4Place q4_place(const Q4MoeArgs& a, uint32_t blocks) {
+    const int n = a.nitems[0], full = a.nitems[1], rest = n - full;
+    const int x = (int)(blockIdx.x % Q4_DIES);
+    const uint32_t slot = blockIdx.x / Q4_DIES, j = slot / blocks;
+    const int f0 = (int)((int64_t)full * x / Q4_DIES), f1 = (int)((int64_t)full * (x + 1) / Q4_DIES);
+    const int r0 = (int)((int64_t)rest * x / Q4_DIES), r1 = (int)((int64_t)rest * (x + 1) / Q4_DIES);
+    const int i = (int)j < f1 - f0 ? f0 + (int)j : full + r0 + (int)j - (f1 - f0);
+    return {i < (((int)j < f1 - f0) ? f1 : full + r1) ? i : -1, slot - j * blocks};
+}
+static unsigned q4_place_blocks(uint32_t max_items, uint32_t blocks) { return Q4_DIES * (max_items / Q4_DIES + 2) * blocks; }
+
 template <bool BF, bool SBF, int GPC, int NT>
-__global__ void __launch_bounds__(Q4_GEMM_THREADS, 2) q4_gateup_gemm_kernel(Q4MoeArgs a) {
+__global__ void __launch_bounds__(Q4_GEMM_THREADS, 2) q4_gateup_gemm_kernel(Q4MoeArgs a, uint32_t blocks) {
     __shared__ __attribute__((aligned(16))) uint8_t lds[q4_gemm_lds<4>()];
-    const Q4Item& it = a.items[blockIdx.y];
-    const int n = *a.nitems, e = it.expert, count = it.count, lane = threadIdx.x & 63;
-    if ((int)blockIdx.y >= n) return;
-    q4_item_gemm<BF, SBF, GPC, NT>(
-        lds, count, a.gu + (size_t)e * a.gu_bytes, (a.width + 7) / 8, a.dims, 1, 0, blockIdx.x, 1u << 24,
+    const Q4Place at = q4_place(a, blocks);
+    if (at.item < 0) return;
+    const Q4Item& it = a.items[at.item];
+    const int e = it.expert, count = it.count, lane = threadIdx.x & 63;
+    q4_item_gemm<BF, SBF, GPC, NT, false>(
+        lds, count, a.gu + (size_t)e * a.gu_bytes, (a.width + 7) / 8, a.dims, 1, 0, at.cb, 1u << 24,
         [&](int i) { return a.x + (size_t)((uint32_t)it.pair[min(i, count - 1)] / a.slots) * a.x_stride; },
+        [&](int i) { return a.xsums + (size_t)((uint32_t)it.pair[min(i, count - 1)] / a.slots) * q4_sum_bytes(a.dims / a.group); },
         [&](uint32_t tile, const auto& v) {
             const uint32_t col = tile * 8 + (lane & 7);
 #pragma unroll
@@ -398,15 +461,17 @@ __global__ void __launch_bounds__(Q4_GEMM_THREADS, 2) q4_gateup_gemm_kernel(Q4Mo
         });
 }
 
-template <bool SBF, int GPC, int NT>
-__global__ void __launch_bounds__(Q4_GEMM_THREADS, 2) q4_down_gemm_kernel(Q4MoeArgs a) {
-    __shared__ __attribute__((aligned(16))) uint8_t lds[q4_gemm_lds<4>()];
-    const Q4Item& it = a.items[blockIdx.y];
-    const int n = *a.nitems, e = it.expert, count = it.count, lane = threadIdx.x & 63;
-    if ((int)blockIdx.y >= n) return;
-    q4_item_gemm<true, SBF, GPC, NT>(
+template <bool SBF, int GPC, int NT, bool RESIDENT>
+__global__ void __launch_bounds__(Q4_GEMM_THREADS, 2) q4_down_gemm_kernel(Q4MoeArgs a, uint32_t blocks) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    const Q4Place at = q4_place(a, blocks);
+    if (at.item < 0) return;
+    const Q4Item& it = a.items[at.item];
+    const int e = it.expert, count = it.count, lane = threadIdx.x & 63;
+    q4_item_gemm<true, SBF, GPC, NT, RESIDENT>(
         lds, count, a.down + (size_t)e * a.down_bytes, q4_tiles(a.dims), a.width, a.terms, (size_t)a.pairs * a.width,
-        blockIdx.x, gridDim.x, [&](int i) { return a.h + (size_t)it.pair[min(i, count - 1)] * a.width; },
+        at.cb, blocks, [&](int i) { return a.h + (size_t)it.pair[min(i, count - 1)] * a.width; },
+        [&](int i) { return a.hsums + (size_t)it.pair[min(i, count - 1)] * q4_sum_bytes(a.width / a.group); },
         [&](uint32_t tile, const auto& v) {
             const uint32_t col = tile * 16 + (lane & 15);
 #pragma unroll
@@ -485,7 +550,7 @@ static void launch_gateup(hipStream_t s, const Q4MoeArgs& a, bool bf, bool sbf, 
 #define DSP 6
 #endif
         else if (a.item == Q4_BIG_ITEM)
-            q4_gateup_gemm_kernel<BF, SBF, GPC, GNT><<<dim3((tiles + 4 * GNT - 1) / (4 * GNT), max_items), Q4_GEMM_THREADS, 0, s>>>(a);
+            q4_gateup_gemm_kernel<BF, SBF, GPC, GNT><<<q4_place_blocks(max_items, (tiles + 4 * GNT - 1) / (4 * GNT)), Q4_GEMM_THREADS, 0, s>>>(a, (tiles + 4 * GNT - 1) / (4 * GNT));
         else if (tiles < 2) q4_gateup_kernel<BF, SBF, GPC, 1, 8, 3, ITEMS><<<dim3(1, max_items), 512, 0, s>>>(a);
         else q4_gateup_kernel<BF, SBF, GPC, 2, 8, 3, ITEMS><<<dim3((tiles + 1) / 2, max_items), 512, 0, s>>>(a);
     });
@@ -500,7 +565,13 @@ static void launch_down(hipStream_t s, const Q4MoeArgs& a, bool sbf, int gpc, ui
             constexpr int GPC = decltype(gpc_)::value;
             if (a.rows == 1) q4_down_one_kernel<SBF, GPC, TERMS, 1, 8, 2><<<tiles, 512, 0, s>>>(a);
             else if (a.item == Q4_BIG_ITEM)
-                q4_down_gemm_kernel<SBF, GPC, DNT2><<<dim3(std::min((tiles + 4 * DNT2 - 1) / (4 * DNT2), (uint32_t)DSP), max_items), Q4_GEMM_THREADS, 0, s>>>(a);
+                [&] {
+                    const uint32_t blocks = std::min((tiles + 4 * DNT2 - 1) / (4 * DNT2), (uint32_t)DSP);
+                    const unsigned grid = q4_place_blocks(max_items, blocks);
+                    const size_t rows = (size_t)TERMS * q4_chunks(a.width) * 4 * 4096;
+                    if (rows <= Q4_RESIDENT_LDS) q4_down_gemm_kernel<SBF, GPC, DNT2, true><<<grid, Q4_GEMM_THREADS, rows, s>>>(a, blocks);
+                    else q4_down_gemm_kernel<SBF, GPC, DNT2, false><<<grid, Q4_GEMM_THREADS, q4_gemm_lds<4>(), s>>>(a, blocks);
+                }();
             else if (tiles >= 4) q4_down_kernel<SBF, GPC, TERMS, 4, 8, 1><<<dim3((tiles + 31) / 32, max_items), 512, 0, s>>>(a);
             else q4_down_kernel<SBF, GPC, TERMS, 1, 4, 1><<<dim3((tiles + 3) / 4, max_items), 256, 0, s>>>(a);
         }
@@ -536,9 +607,11 @@ static size_t q4_carve(ea_q4_scratch* s, uint64_t base, const ea_q4_experts* ex,
         return p;
     };
     s->items = take(sizeof(Q4Item) * q4_max_items(ex->count, pairs));
-    s->count = take(4);
+    s->count = take(8);
     s->h = take(3 * 2 * pairs * ex->width);
     s->y = take(4 * (size_t)pairs * ex->dims);
+    s->sums = take((size_t)rows * q4_sum_bytes(ex->dims / 32) + 64);
+    s->hsums = take(pairs * q4_sum_bytes(ex->width / 32) + 64);
     s->rows = rows;
     s->slots = slots;
     return at;
@@ -597,6 +670,10 @@ int ea_q4_routed(ea_stream_t stream, const void* x, int x_dtype, uint32_t x_stri
     a.items = dptr<Q4Item>(sc->items);
     a.h = dptr<uint16_t>(sc->h);
     a.y = dptr<float>(sc->y);
+    a.xsums = dptr<uint8_t>(sc->sums);
+    a.hsums = dptr<uint8_t>(sc->hsums);
+    a.group = ex->group;
+    a.bf = x_dtype == BF16;
     a.out = out;
     a.rows = R;
     a.pairs = R * sc->slots;
@@ -613,8 +690,10 @@ int ea_q4_routed(ea_stream_t stream, const void* x, int x_dtype, uint32_t x_stri
     const uint32_t max_items = q4_max_items(a.experts, a.pairs, a.item);
     hipStream_t s = as_stream(stream);
     const bool sbf = ex->s_dtype == BF16;
-    if (R > Q4_ROWS) q4_group_kernel<<<1, 1024, 0, s>>>(a);
+    const bool big = a.item == Q4_BIG_ITEM;
+    if (R > Q4_ROWS) q4_group_kernel<<<1 + (big ? (R + 15) / 16 : 0), 1024, 0, s>>>(a);
     launch_gateup(s, a, x_dtype == BF16, sbf, gpc, max_items);
+    if (big) q4_hsums_kernel<<<(a.pairs + 3) / 4, 256, 0, s>>>(a);
     if (a.terms == 1) launch_down<1>(s, a, sbf, gpc, max_items);
     else if (a.terms == 2) launch_down<2>(s, a, sbf, gpc, max_items);
     else launch_down<3>(s, a, sbf, gpc, max_items);

@@ -11,10 +11,12 @@ namespace ea {
 constexpr int Q4_GEMM_THREADS = 256;
 template <int MT>
 constexpr int q4_gemm_lds() { return 2 * MT * 16 * 256; }
+constexpr int Q4_RESIDENT_LDS = 65536;
 
 // One chunk from LDS: row r of the block at 256 r, its 16-byte piece q at 16 (q ^ (r & 15)), so that the 16 rows of an
-// operand's quarter lie in different banks.
-template <bool BF, bool SBF, int GPC, int MT, int NT>
+// operand's quarter lie in different banks. With BIAS the groups' biases are applied here, from sums of x that are made here
+// too; without, out gets the scaled sums alone.
+template <bool BF, bool SBF, int GPC, int MT, int NT, bool BIAS>
 __device__ __forceinline__ void q4_gemm_chunk(const uint8_t* lds, const u4v (&words)[NT], const Q4Params<GPC> (&par)[NT],
                                               int lane, f4v (&out)[NT][MT]) {
     constexpr int JPG = 4 / GPC;
@@ -29,10 +31,12 @@ __device__ __forceinline__ void q4_gemm_chunk(const uint8_t* lds, const u4v (&wo
             for (int j = 0; j < JPG; ++j)
                 a[mt][j] = *reinterpret_cast<const u4v*>(lds + (mt * 16 + r) * 256 + 16 * ((4 * (g * JPG + j) + quad) ^ r));
         f4v xs[MT];
+        if constexpr (BIAS) {
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+            for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-            for (int j = 0; j < JPG; ++j) xs[mt] = q4_mfma<BF>(a[mt][j], q4_ones<BF>(), j ? xs[mt] : zero);
+                for (int j = 0; j < JPG; ++j) xs[mt] = q4_mfma<BF>(a[mt][j], q4_ones<BF>(), j ? xs[mt] : zero);
+        }
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             f4v acc[MT];
@@ -47,34 +51,118 @@ __device__ __forceinline__ void q4_gemm_chunk(const uint8_t* lds, const u4v (&wo
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    out[t][mt][i] = __builtin_fmaf(b, xs[mt][i], __builtin_fmaf(s, acc[mt][i], out[t][mt][i]));
+                for (int i = 0; i < 4; ++i) {
+                    const float v = __builtin_fmaf(s, acc[mt][i], out[t][mt][i]);
+                    out[t][mt][i] = BIAS ? __builtin_fmaf(b, xs[mt][i], v) : v;
+                }
+        }
+    }
+}
+
+// ---- the biases of all groups at once -----------------------------------------------------------------------------------
+// Where the rows' sums over each group are known before, biases need no fp32 operations of their own: sums and biases are a
+// product over the groups. A sum is held as three bf16 numbers that add up to it (24 bits), for each eight groups 64 bytes: the
+// eight first terms, the second, the third, zeros; so a lane's A operand of eight groups is one 16-byte read (lanes 16 q .. are
+// term q), the B operand the eight biases, the same for every term, collected from the chunks' parameters as they pass. (Half
+// of the loop's fp32 operations went into the biases before, and with four tiles a wave a fifth of its matrix instructions.)
+__host__ __device__ inline uint32_t q4_sum_bytes(uint32_t groups) { return (groups + 7) / 8 * 64; }
+
+template <bool SBF, int GPC>
+struct Q4Biases {
+    u4v hi, lo;  // eight biases in bf16, the last ones at the end; fp16's 11 bits as two of them
+
+    __device__ __forceinline__ void shift(uint32_t h, uint32_t l) {  // two biases, or one in the low half
+        if constexpr (GPC == 1) {
+            hi = u4v{__builtin_amdgcn_alignbit(hi[1], hi[0], 16), __builtin_amdgcn_alignbit(hi[2], hi[1], 16),
+                     __builtin_amdgcn_alignbit(hi[3], hi[2], 16), __builtin_amdgcn_alignbit(h, hi[3], 16)};
+            if constexpr (!SBF)
+                lo = u4v{__builtin_amdgcn_alignbit(lo[1], lo[0], 16), __builtin_amdgcn_alignbit(lo[2], lo[1], 16),
+                         __builtin_amdgcn_alignbit(lo[3], lo[2], 16), __builtin_amdgcn_alignbit(l, lo[3], 16)};
+        } else {
+            hi = u4v{hi[1], hi[2], hi[3], h};
+            if constexpr (!SBF) lo = u4v{lo[1], lo[2], lo[3], l};
+        }
+    }
+    // A chunk's biases.
+    __device__ __forceinline__ void take(const Q4Params<GPC>& par) {
+#pragma unroll
+        for (int g = 0; g < GPC; g += 2) {
+            const uint32_t w0 = par.w[g], w1 = GPC == 1 ? 0u : par.w[g + (GPC > 1)];
+            if constexpr (SBF) {
+                shift((w0 >> 16) | (w1 & 0xffff0000u), 0);
+            } else {
+                const float a = h2f((uint16_t)(w0 >> 16)), b = h2f((uint16_t)(w1 >> 16));
+                const uint16_t ah = f2bf(a), bh = f2bf(b);
+                shift((uint32_t)ah | (uint32_t)bh << 16, (uint32_t)f2bf(a - bf2f(ah)) | (uint32_t)f2bf(b - bf2f(bh)) << 16);
+            }
+        }
+    }
+    template <int MT>
+    __device__ __forceinline__ void add(const u4v (&sums)[MT], f4v (&out)[MT]) const {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            out[mt] = q4_mfma<true>(sums[mt], hi, out[mt]);
+            if constexpr (!SBF) out[mt] = q4_mfma<true>(sums[mt], lo, out[mt]);
+        }
+    }
+};
+
+// A row's sums over its groups, in that form: a wave a row, eight values a lane; `terms` of the row, `plane` values apart.
+template <bool BF>
+__device__ __forceinline__ void q4_row_sums(const uint16_t* row, uint32_t terms, size_t plane, uint32_t k, uint32_t group,
+                                            uint8_t* to, int lane) {
+    const uint32_t groups = k / group, per = group / 8, padded = (groups + 7) / 8 * 8;
+    for (uint32_t p = lane; p - lane < padded * per; p += 64) {  // a piece of eight values
+        float v = 0.0f;
+        if (p < k / 8)
+            for (uint32_t t = 0; t < terms; ++t) {
+                const u4v u = *reinterpret_cast<const u4v_a8*>(row + t * plane + 8 * p);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    v = v + (BF ? bf2f((uint16_t)(u[i] & 0xffffu)) : h2f((uint16_t)(u[i] & 0xffffu)));
+                    v = v + (BF ? bf2f((uint16_t)(u[i] >> 16)) : h2f((uint16_t)(u[i] >> 16)));
+                }
+            }
+        v = v + lane_xor<1>(v);
+        v = v + lane_xor<2>(v);
+        if (per >= 8) v = v + lane_xor<4>(v);
+        if (per >= 16) v = v + lane_xor<8>(v);
+        const uint32_t g = p / per;
+        if (p % per == 0 && g < padded) {
+            uint16_t* o = reinterpret_cast<uint16_t*>(to + (size_t)(g / 8) * 64) + (g & 7);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const uint16_t b = t < 3 ? f2bf(v) : 0;
+                o[8 * t] = b;
+                v = __builtin_fabsf(v) < __builtin_inff() ? v - bf2f(b) : 0.0f;
+            }
         }
     }
 }
 
 // The column blocks cb, cb + cb_step, .. of W (its first tile at w) times the block's rows. row(i): row i's activations,
-// terms of them `plane` values apart (their products add up). store(tile, sums of its 16 MT rows).
-template <bool BF, bool SBF, int GPC, int MT, int NT, typename ROW, typename STORE>
+// terms of them `plane` values apart (their products add up); sums(i): its groups' sums, for the biases, or with BIAS null.
+// store(tile, sums of its 16 MT rows). RESIDENT: all of the rows' terms and chunks lie in LDS at once (at most 64 KB, the
+// size of lds then), so that after the first barrier the waves go on alone; else two chunks do.
+template <bool BF, bool SBF, int GPC, int MT, int NT, bool BIAS, bool RESIDENT, typename ROW, typename SUMS, typename STORE>
 __device__ __forceinline__ void q4_gemm(uint8_t* lds, const uint8_t* w, uint32_t tiles, uint32_t k, uint32_t terms,
-                                        size_t plane, uint32_t cb, uint32_t cb_step, ROW row, STORE store) {
+                                        size_t plane, uint32_t cb, uint32_t cb_step, ROW row, SUMS sums, STORE store) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t chunks = q4_chunks(k), piece = threadIdx.x & 15, row0 = threadIdx.x >> 4;
-    const size_t tile_bytes = (size_t)chunks * q4_chunk_bytes(GPC);
+    const uint32_t tile_bytes = chunks * q4_chunk_bytes(GPC);
+    constexpr uint32_t CYCLE = 8 / GPC;  // chunks of eight groups
     const uint16_t* src[MT];
+    const uint8_t* rs[MT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) src[i] = row(row0 + 16 * i);
+    for (int i = 0; i < MT; ++i) {
+        src[i] = row(row0 + 16 * i);
+        if constexpr (!BIAS) rs[i] = sums(16 * i + (lane & 15)) + 16 * (lane >> 4);
+    }
     const uint32_t to = row0 * 256 + 16 * (piece ^ row0);  // row0 + 16 i: 4096 bytes further each
-    u4v ra[MT], rw[NT];
-    Q4Params<GPC> rp[NT];
-    const auto load = [&](uint32_t cb_, uint32_t term, uint32_t c) {
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            const uint32_t tile = min((cb_ * 4 + wave) * NT + t, tiles - 1);
-            const uint8_t* p = w + tile * tile_bytes + (size_t)c * q4_chunk_bytes(GPC);
-            rw[t] = reinterpret_cast<const u4v*>(p)[lane];
-            rp[t] = q4_params<GPC>(p, lane);
-        }
+    u4v ra[MT], rw[2][NT], rx[MT];
+    Q4Params<GPC> rp[2][NT];
+    Q4Biases<SBF, GPC> biases[NT];
+    const auto load_rows = [&](uint32_t term, uint32_t c) {
         // past k, where the weights are zeros, the row's last 32 values again
         const uint32_t at = c * Q4_CHUNK + 8 * piece, off = at < k ? at : k - 32 + 8 * (piece & 3);
 #pragma unroll
@@ -84,27 +172,53 @@ __device__ __forceinline__ void q4_gemm(uint8_t* lds, const uint8_t* w, uint32_t
 #pragma unroll
         for (int i = 0; i < MT; ++i) *reinterpret_cast<u4v*>(lds + buffer * (MT * 4096) + to + 4096 * i) = ra[i];
     };
+    const auto load = [&](int set, uint32_t cb_, uint32_t term, uint32_t c) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const uint32_t tile = min((cb_ * 4 + wave) * NT + t, tiles - 1);
+            const uint8_t* p = w + (size_t)tile * tile_bytes + (size_t)c * q4_chunk_bytes(GPC);
+            rw[set][t] = reinterpret_cast<const u4v*>(p)[lane];
+            rp[set][t] = q4_params<GPC>(p, lane);
+        }
+        if constexpr (!RESIDENT) load_rows(term, c);
+    };
     f4v out[NT][MT];
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) out[t][mt] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
-    uint32_t c = 0, term = 0, buffer = 0;
-    load(cb, 0, 0);
-    stage(0);
-    for (;;) {
+    uint32_t c = 0, term = 0;
+    // one chunk; false after the last
+    const auto step = [&](auto set_) __attribute__((always_inline)) {
+        constexpr int SET = decltype(set_)::value;
+        if constexpr (!RESIDENT) stage(SET);
         const bool ends = c + 1 == chunks && term + 1 == terms;  // of the column block
         uint32_t nc = c + 1, nterm = term, ncb = cb;
         if (nc == chunks) nc = 0, ++nterm;
         if (nterm == terms) nterm = 0, ncb += cb_step;
         const bool more = ncb * 4 * NT < tiles;
-        u4v words[NT];
-        Q4Params<GPC> par[NT];
+        if constexpr (!BIAS)
+            if (term == 0 && c % CYCLE == 0)
 #pragma unroll
-        for (int t = 0; t < NT; ++t) words[t] = rw[t], par[t] = rp[t];
-        if (more) load(ncb, nterm, nc);
-        __syncthreads();  // the chunk is staged, and the buffer of the one before it is free
-        q4_gemm_chunk<BF, SBF, GPC, MT, NT>(lds + buffer * (MT * 4096), words, par, lane, out);
+                for (int mt = 0; mt < MT; ++mt) rx[mt] = *reinterpret_cast<const u4v*>(rs[mt] + c / CYCLE * 64);
+        if (more) load(1 - SET, ncb, nterm, nc);
+        if constexpr (!RESIDENT) __syncthreads();  // the chunk is staged; its buffer's last readers were before the last one
+        q4_gemm_chunk<BF, SBF, GPC, MT, NT, BIAS>(lds + (RESIDENT ? term * chunks + c : SET) * (MT * 4096), rw[SET], rp[SET],
+                                                  lane, out);
+        if constexpr (!BIAS)
+            if (term == 0) {
+#pragma unroll
+                for (int t = 0; t < NT; ++t) biases[t].take(rp[SET][t]);
+                if (c % CYCLE == CYCLE - 1 || nc == 0) {
+                    for (uint32_t i = c % CYCLE; i < CYCLE - 1; ++i) {  // no more chunks: zeros up to the eighth group
+                        constexpr Q4Params<GPC> none{};
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) biases[t].take(none);
+                    }
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) biases[t].add(rx, out[t]);
+                }
+            }
         if (ends) {
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
@@ -114,12 +228,21 @@ __device__ __forceinline__ void q4_gemm(uint8_t* lds, const uint8_t* w, uint32_t
                 for (int mt = 0; mt < MT; ++mt) out[t][mt] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
             }
         }
-        if (!more) break;
-        buffer ^= 1;
-        stage(buffer);
         c = nc;
         term = nterm;
         cb = ncb;
+        return more;
+    };
+    load(0, cb, 0, 0);
+    if constexpr (RESIDENT) {
+        for (uint32_t t = 0; t < terms; ++t)
+            for (uint32_t ci = 0; ci < chunks; ++ci) {
+                load_rows(t, ci);
+                stage(t * chunks + ci);
+            }
+        __syncthreads();
+    }
+    while (step(std::integral_constant<int, 0>{}) && step(std::integral_constant<int, 1>{})) {
     }
 }
 

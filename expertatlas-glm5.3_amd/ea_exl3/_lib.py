@@ -84,7 +84,8 @@ class Q4Experts(C.Structure):
 
 
 class Q4Scratch(C.Structure):
-    _fields_ = [("items", U64), ("count", U64), ("h", U64), ("y", U64), ("rows", U32), ("slots", U32),
+    _fields_ = [("items", U64), ("count", U64), ("h", U64), ("y", U64), ("sums", U64), ("hsums", U64),
+                ("rows", U32), ("slots", U32),
                 ("experts", U32), ("dims", U32), ("width", U32), ("reserved", U32)]
 
 

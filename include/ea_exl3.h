@@ -344,7 +344,7 @@ typedef struct ea_q4_experts {
 /* Scratch for calls of up to `rows` rows with `slots` slots a row, carved from one device buffer (256-byte aligned). It needs
  * no clearing and may serve layers of no more experts, dims and width in turn; calls that overlap on one scratch race. */
 typedef struct ea_q4_scratch {
-    uint64_t items, count, h, y;
+    uint64_t items, count, h, y, sums, hsums;
     uint32_t rows, slots, experts, dims, width, reserved;
 } ea_q4_scratch;
 size_t ea_q4_scratch_bytes(const ea_q4_experts* ex, uint32_t rows, uint32_t slots);
