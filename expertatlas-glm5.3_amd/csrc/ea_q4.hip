@@ -106,26 +106,28 @@ __global__ void __launch_bounds__(64 * WK) q4_linear_kernel(Q4LinArgs a) {
     }
 }
 
+#ifndef LV
+#define LV 2
+#endif
+#ifndef LAH
+#define LAH 1
+#endif
 // More rows: 16 MT rows and 4 NT tiles a block.
 template <bool BF, bool SBF, int GPC, int MT, int NT>
 __global__ void __launch_bounds__(Q4_GEMM_THREADS, 2) q4_linear_gemm_kernel(Q4LinArgs a) {
-    __shared__ __attribute__((aligned(16))) uint8_t lds[q4_gemm_lds<MT>()];
+    __shared__ __attribute__((aligned(16))) uint8_t lds[q4_gemm_lds<MT, NT>()];
     const Q4Job job = a.job[blockIdx.z];
     const uint32_t tiles = q4_tiles(job.n), m0 = blockIdx.y * 16 * MT;
     if (blockIdx.x * 4 * NT >= tiles) return;
     const int lane = threadIdx.x & 63;
-    q4_gemm<BF, SBF, GPC, MT, NT, true, false>(
+    q4_gemm<BF, SBF, GPC, MT, NT, true, false, LAH>(
         lds, job.w, tiles, a.k, 1, 0, blockIdx.x, 1u << 24,
         [&](uint32_t i) { return a.x + (size_t)min(m0 + i, a.m - 1) * a.x_stride; }, nullptr,
-        [&](uint32_t tile, const f4v(&v)[MT]) {
-            const uint32_t n = tile * 16 + (lane & 15);
+        [&](uint32_t r, uint32_t n, const f4v& v) {
+            if (m0 + r >= a.m) return;
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t r = m0 + 16 * mt + 4 * (lane >> 4) + i;
-                    if (r < a.m && n < job.n) store_act(job.y, job.y_dtype, (size_t)r * job.n + n, v[mt][i]);
-                }
+            for (int i = 0; i < 4; ++i)
+                if (n + i < job.n) store_act(job.y, job.y_dtype, (size_t)(m0 + r) * job.n + n + i, v[i]);
         });
 }
 
@@ -138,9 +140,7 @@ static int launch_linear(hipStream_t s, const Q4LinArgs& a, uint32_t tiles, bool
             if (tiles * jobs < 512) q4_linear_kernel<BF, SBF, GPC, 1, 1, 16, 3><<<dim3(tiles, 1, jobs), 1024, 0, s>>>(a);
             else q4_linear_kernel<BF, SBF, GPC, 1, 2, 8, 3><<<dim3((tiles + 1) / 2, 1, jobs), 512, 0, s>>>(a);
         } else {
-#ifndef LV
-#define LV 2
-#endif
+
             if (LV == 0) q4_linear_kernel<BF, SBF, GPC, 4, 1, 8, 1><<<dim3(tiles, (a.m + 63) / 64, jobs), 512, 0, s>>>(a);
             else q4_linear_gemm_kernel<BF, SBF, GPC, 4, LV ? LV : 1><<<dim3((tiles + 4 * LV - 1) / (4 * (LV ? LV : 1)), (a.m + 63) / 64, jobs), Q4_GEMM_THREADS, 0, s>>>(a);
         }

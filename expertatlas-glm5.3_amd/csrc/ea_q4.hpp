@@ -167,6 +167,29 @@ __device__ __forceinline__ float q4_total(const f4v (&part)[WK][NT][MT][64], int
     return v;
 }
 
+// The sums of NT tiles (lane l: rows 4 (l >> 4) + i, column l & 15 of each) through a wave's own LDS, so that a lane gets four
+// neighbouring columns: piece(row, column, four sums) for 16 rows of 16 NT columns, 16 NT / 4 lanes a row. A store then covers
+// whole lines, and a wave has a quarter of the stores in flight.
+template <int NT>
+constexpr int q4_turn_floats() { return 16 * (16 * NT + 4); }
+template <int NT, typename F>
+__device__ __forceinline__ void q4_turn(float* lds, const f4v (&v)[NT], int lane, F piece) {
+    constexpr int STRIDE = 16 * NT + 4, LANES = 4 * NT;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) lds[(4 * (lane >> 4) + i) * STRIDE + 16 * t + (lane & 15)] = v[t][i];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the wave's LDS works in order; the compiler has to as well
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int k = 0; k < NT; ++k) {
+        const int at = 64 * k + lane, r = at / LANES, c = 4 * (at % LANES);
+        piece(r, c, *reinterpret_cast<const f4v*>(lds + r * STRIDE + c));
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // f(groups a chunk, x in bf16, scales in bf16) as compile-time constants.
 template <typename F>
 inline void q4_types(bool bf, bool sbf, int gpc, F f) {

@@ -199,6 +199,20 @@ __device__ __forceinline__ void store_terms(uint16_t* h, int terms, size_t plane
     }
 }
 
+// Four neighbouring ones.
+__device__ __forceinline__ void store_terms4(uint16_t* h, int terms, size_t plane, size_t at, f4v v) {
+    for (int i = 0; i < terms; ++i) {
+        uint16_t b[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            b[k] = f2bf(v[k]);
+            v[k] = __builtin_fabsf(v[k]) < __builtin_inff() ? v[k] - bf2f(b[k]) : 0.0f;
+        }
+        *reinterpret_cast<u2v*>(h + (size_t)i * plane + at) =
+            u2v{(uint32_t)b[0] | (uint32_t)b[1] << 16, (uint32_t)b[2] | (uint32_t)b[3] << 16};
+    }
+}
+
 // ---- gate | up ------------------------------------------------------------------------------------------------------
 // Block (NT tiles of gate | up, item): 16 rows of a matrix instruction, those that the item does not have as zeros, which
 // cost neither loads nor cache; WK waves take every WK-th chunk. Up to 16 rows nothing is sorted before: block (tiles, pair)
@@ -357,8 +371,9 @@ __global__ void __launch_bounds__(64 * WK) q4_down_one_kernel(Q4MoeArgs a) {
 template <bool SBF, int GPC, int TERMS, int NT, int WK, int NB>
 __global__ void __launch_bounds__(64 * WK) q4_down_kernel(Q4MoeArgs a) {
     constexpr int PER = TERMS == 1 ? 16 : TERMS == 2 ? 8 : 4;  // pairs a product
+    __shared__ float turn[WK][q4_turn_floats<NT>()];
     const Q4Item& it = a.items[blockIdx.y];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quad = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = *a.nitems, e = it.expert, count = it.count;
     const int from = it.pair[lane & (PER - 1)];
     if ((int)blockIdx.y >= n) return;
@@ -370,11 +385,6 @@ __global__ void __launch_bounds__(64 * WK) q4_down_kernel(Q4MoeArgs a) {
         const uint16_t* row[1] = {nullptr};
         if (m0 + (lane & (PER - 1)) < count && term < TERMS)
             row[0] = a.h + term * plane + (size_t)(m0 ? it.pair[m0 + (lane & (PER - 1))] : from) * a.width;
-        // the pairs of this lane's sums: value i is pair 4 (quad mod PER / 4) + i
-        const int at0 = m0 + 4 * (quad & (PER / 4 - 1));
-        int to[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) to[i] = it.pair[at0 + i];
         const uint32_t mine = (blockIdx.x * WK + wave) * NT;
         if (mine < tiles) {
             const uint32_t tile0 = min(mine, tiles - NT);  // the last wave's tiles overlap
@@ -383,16 +393,20 @@ __global__ void __launch_bounds__(64 * WK) q4_down_kernel(Q4MoeArgs a) {
             for (int t = 0; t < NT; ++t) out[t][0] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
             q4_stream<true, SBF, GPC, 1, NT, NB, true>(w + tile0 * tile_bytes, tile_bytes, 0, 1, chunks, row, a.width, lane,
                                                   out);
+            f4v v[NT];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    float v = out[t][0][i];
-                    if constexpr (TERMS == 3) v = v + lane_xor<16>(v);
-                    if constexpr (TERMS >= 2) v = v + lane_xor<32>(v);
-                    const uint32_t col = (tile0 + t) * 16 + (lane & 15);
-                    if (at0 + i < count && quad < PER / 4 && col < a.dims) a.y[(size_t)to[i] * a.dims + col] = v;
+                for (int i = 0; i < 4; ++i) {
+                    v[t][i] = out[t][0][i];
+                    if constexpr (TERMS == 3) v[t][i] = v[t][i] + lane_xor<16>(v[t][i]);
+                    if constexpr (TERMS >= 2) v[t][i] = v[t][i] + lane_xor<32>(v[t][i]);
                 }
+            q4_turn<NT>(turn[wave], v, lane, [&](int r, int c, const f4v& p) {
+                const uint32_t col = tile0 * 16 + c;
+                if (r < PER && m0 + r < count && col < a.dims)
+                    *reinterpret_cast<f4v*>(a.y + (size_t)it.pair[m0 + r] * a.dims + col) = p;
+            });
         }
     }
 }
@@ -405,15 +419,22 @@ __global__ void __launch_bounds__(256) q4_hsums_kernel(Q4MoeArgs a) {
                           a.hsums + (size_t)i * q4_sum_bytes(a.width / a.group), threadIdx.x & 63);
 }
 
+#ifndef WPS
+#define WPS 2
+#endif
+#ifndef GAH
+#define GAH 1
+#define DAH 1
+#endif
 // ---- long items -----------------------------------------------------------------------------------------------------
 // An item's products by q4_gemm, with as many row groups as it has.
-template <bool BF, bool SBF, int GPC, int NT, bool RESIDENT, typename ROW, typename SUMS, typename STORE>
+template <bool BF, bool SBF, int GPC, int NT, bool RESIDENT, int AHEAD, typename ROW, typename SUMS, typename STORE>
 __device__ __forceinline__ void q4_item_gemm(uint8_t* lds, int count, const uint8_t* w, uint32_t tiles, uint32_t k,
                                              uint32_t terms, size_t plane, uint32_t cb, uint32_t cb_step, ROW row,
                                              SUMS sums, STORE store) {
-    if (count <= 16) q4_gemm<BF, SBF, GPC, 1, NT, false, RESIDENT>(lds, w, tiles, k, terms, plane, cb, cb_step, row, sums, store);
-    else if (count <= 32) q4_gemm<BF, SBF, GPC, 2, NT, false, RESIDENT>(lds, w, tiles, k, terms, plane, cb, cb_step, row, sums, store);
-    else q4_gemm<BF, SBF, GPC, 4, NT, false, RESIDENT>(lds, w, tiles, k, terms, plane, cb, cb_step, row, sums, store);
+    if (count <= 16) q4_gemm<BF, SBF, GPC, 1, NT, false, RESIDENT, AHEAD>(lds, w, tiles, k, terms, plane, cb, cb_step, row, sums, store);
+    else if (count <= 32) q4_gemm<BF, SBF, GPC, 2, NT, false, RESIDENT, AHEAD>(lds, w, tiles, k, terms, plane, cb, cb_step, row, sums, store);
+    else q4_gemm<BF, SBF, GPC, 4, NT, false, RESIDENT, AHEAD>(lds, w, tiles, k, terms, plane, cb, cb_step, row, sums, store);
 }
 
 // Blocks go to the card's eight dies in turn, and each die has an L2 of its own: die x takes the x-th eighth of the full items
@@ -436,51 +457,42 @@ __device__ __forceinline__ Q4Place q4_place(const Q4MoeArgs& a, uint32_t blocks)
 static unsigned q4_place_blocks(uint32_t max_items, uint32_t blocks) { return Q4_DIES * (max_items / Q4_DIES + 2) * blocks; }
 
 template <bool BF, bool SBF, int GPC, int NT>
-__global__ void __launch_bounds__(Q4_GEMM_THREADS, 2) q4_gateup_gemm_kernel(Q4MoeArgs a, uint32_t blocks) {
-    __shared__ __attribute__((aligned(16))) uint8_t lds[q4_gemm_lds<4>()];
+__global__ void __launch_bounds__(Q4_GEMM_THREADS, WPS) q4_gateup_gemm_kernel(Q4MoeArgs a, uint32_t blocks) {
+    __shared__ __attribute__((aligned(16))) uint8_t lds[q4_gemm_lds<4, NT>()];
     const Q4Place at = q4_place(a, blocks);
     if (at.item < 0) return;
     const Q4Item& it = a.items[at.item];
-    const int e = it.expert, count = it.count, lane = threadIdx.x & 63;
-    q4_item_gemm<BF, SBF, GPC, NT, false>(
+    const int e = it.expert, count = it.count;
+    q4_item_gemm<BF, SBF, GPC, NT, false, GAH>(
         lds, count, a.gu + (size_t)e * a.gu_bytes, (a.width + 7) / 8, a.dims, 1, 0, at.cb, 1u << 24,
         [&](int i) { return a.x + (size_t)((uint32_t)it.pair[min(i, count - 1)] / a.slots) * a.x_stride; },
         [&](int i) { return a.xsums + (size_t)((uint32_t)it.pair[min(i, count - 1)] / a.slots) * q4_sum_bytes(a.dims / a.group); },
-        [&](uint32_t tile, const auto& v) {
-            const uint32_t col = tile * 8 + (lane & 7);
+        [&](int m, uint32_t c, const f4v& v) {  // columns 0 .. 7 of 16 are the gate's, the others the up projection's
+            const uint32_t col = c / 16 * 8 + c % 8;
+            f4v u;
 #pragma unroll
-            for (int mt = 0; mt < (int)(sizeof(v) / sizeof(f4v)); ++mt)
+            for (int i = 0; i < 4; ++i) u[i] = lane_xor<2>(v[i]);
+            if ((c & 8) || m >= count || col >= a.width) return;
+            f4v h;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float u = lane_xor<8>(v[mt][i]);  // lanes 0 .. 7 of 16 have the gate, the others the up column
-                    const int m = 16 * mt + 4 * (lane >> 4) + i;
-                    if ((lane & 8) || m >= count || col >= a.width) continue;
-                    store_terms(a.h, a.terms, (size_t)a.pairs * a.width, (size_t)it.pair[m] * a.width + col,
-                                swiglu(v[mt][i], u));
-                }
+            for (int i = 0; i < 4; ++i) h[i] = swiglu(v[i], u[i]);
+            store_terms4(a.h, a.terms, (size_t)a.pairs * a.width, (size_t)it.pair[m] * a.width + col, h);
         });
 }
 
 template <bool SBF, int GPC, int NT, bool RESIDENT>
-__global__ void __launch_bounds__(Q4_GEMM_THREADS, 2) q4_down_gemm_kernel(Q4MoeArgs a, uint32_t blocks) {
+__global__ void __launch_bounds__(Q4_GEMM_THREADS, WPS) q4_down_gemm_kernel(Q4MoeArgs a, uint32_t blocks) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const Q4Place at = q4_place(a, blocks);
     if (at.item < 0) return;
     const Q4Item& it = a.items[at.item];
-    const int e = it.expert, count = it.count, lane = threadIdx.x & 63;
-    q4_item_gemm<true, SBF, GPC, NT, RESIDENT>(
+    const int e = it.expert, count = it.count;
+    q4_item_gemm<true, SBF, GPC, NT, RESIDENT, DAH>(
         lds, count, a.down + (size_t)e * a.down_bytes, q4_tiles(a.dims), a.width, a.terms, (size_t)a.pairs * a.width,
         at.cb, blocks, [&](int i) { return a.h + (size_t)it.pair[min(i, count - 1)] * a.width; },
         [&](int i) { return a.hsums + (size_t)it.pair[min(i, count - 1)] * q4_sum_bytes(a.width / a.group); },
-        [&](uint32_t tile, const auto& v) {
-            const uint32_t col = tile * 16 + (lane & 15);
-#pragma unroll
-            for (int mt = 0; mt < (int)(sizeof(v) / sizeof(f4v)); ++mt)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int m = 16 * mt + 4 * (lane >> 4) + i;
-                    if (m < count && col < a.dims) a.y[(size_t)it.pair[m] * a.dims + col] = v[mt][i];
-                }
+        [&](int m, uint32_t col, const f4v& v) {
+            if (m < count && col < a.dims) *reinterpret_cast<f4v*>(a.y + (size_t)it.pair[m] * a.dims + col) = v;
         });
 }
 
@@ -568,9 +580,10 @@ static void launch_down(hipStream_t s, const Q4MoeArgs& a, bool sbf, int gpc, ui
                 [&] {
                     const uint32_t blocks = std::min((tiles + 4 * DNT2 - 1) / (4 * DNT2), (uint32_t)DSP);
                     const unsigned grid = q4_place_blocks(max_items, blocks);
-                    const size_t rows = (size_t)TERMS * q4_chunks(a.width) * 4 * 4096;
-                    if (rows <= Q4_RESIDENT_LDS) q4_down_gemm_kernel<SBF, GPC, DNT2, true><<<grid, Q4_GEMM_THREADS, rows, s>>>(a, blocks);
-                    else q4_down_gemm_kernel<SBF, GPC, DNT2, false><<<grid, Q4_GEMM_THREADS, q4_gemm_lds<4>(), s>>>(a, blocks);
+                    const uint32_t buffers = TERMS * q4_chunks(a.width);
+                    if (buffers <= Q4_RESIDENT)
+                        q4_down_gemm_kernel<SBF, GPC, DNT2, true><<<grid, Q4_GEMM_THREADS, q4_gemm_lds<4, DNT2>(buffers), s>>>(a, blocks);
+                    else q4_down_gemm_kernel<SBF, GPC, DNT2, false><<<grid, Q4_GEMM_THREADS, q4_gemm_lds<4, DNT2>(), s>>>(a, blocks);
                 }();
             else if (tiles >= 4) q4_down_kernel<SBF, GPC, TERMS, 4, 8, 1><<<dim3((tiles + 31) / 32, max_items), 512, 0, s>>>(a);
             else q4_down_kernel<SBF, GPC, TERMS, 1, 4, 1><<<dim3((tiles + 3) / 4, max_items), 256, 0, s>>>(a);

@@ -9,9 +9,11 @@
 namespace ea {
 
 constexpr int Q4_GEMM_THREADS = 256;
-template <int MT>
-constexpr int q4_gemm_lds() { return 2 * MT * 16 * 256; }
-constexpr int Q4_RESIDENT_LDS = 65536;
+// LDS: `buffers` chunks of 16 MT rows, 4096 MT bytes each, two buffers of their sums over eight groups, 1024 MT each, and the
+// waves' places to turn their sums.
+template <int MT, int NT>
+constexpr int q4_gemm_lds(int buffers = 2) { return buffers * MT * 4096 + 2 * MT * 1024 + 4 * 4 * q4_turn_floats<NT>(); }
+constexpr int Q4_RESIDENT = 4;  // chunks of all terms that stay in LDS at most
 
 // One chunk from LDS: row r of the block at 256 r, its 16-byte piece q at 16 (q ^ (r & 15)), so that the 16 rows of an
 // operand's quarter lie in different banks. With BIAS the groups' biases are applied here, from sums of x that are made here
@@ -142,9 +144,10 @@ __device__ __forceinline__ void q4_row_sums(const uint16_t* row, uint32_t terms,
 
 // The column blocks cb, cb + cb_step, .. of W (its first tile at w) times the block's rows. row(i): row i's activations,
 // terms of them `plane` values apart (their products add up); sums(i): its groups' sums, for the biases, or with BIAS null.
-// store(tile, sums of its 16 MT rows). RESIDENT: all of the rows' terms and chunks lie in LDS at once (at most 64 KB, the
-// size of lds then), so that after the first barrier the waves go on alone; else two chunks do.
-template <bool BF, bool SBF, int GPC, int MT, int NT, bool BIAS, bool RESIDENT, typename ROW, typename SUMS, typename STORE>
+// store(row, column of W's packed rows, the sums of four columns). RESIDENT: all of the rows' terms and chunks lie in LDS at once (Q4_RESIDENT of
+// them at most), so that after the first barrier the waves go on alone; else two chunks do. Weights are read AHEAD (1 or
+// 2) chunks before their products.
+template <bool BF, bool SBF, int GPC, int MT, int NT, bool BIAS, bool RESIDENT, int AHEAD, typename ROW, typename SUMS, typename STORE>
 __device__ __forceinline__ void q4_gemm(uint8_t* lds, const uint8_t* w, uint32_t tiles, uint32_t k, uint32_t terms,
                                         size_t plane, uint32_t cb, uint32_t cb_step, ROW row, SUMS sums, STORE store) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -152,16 +155,26 @@ __device__ __forceinline__ void q4_gemm(uint8_t* lds, const uint8_t* w, uint32_t
     const uint32_t tile_bytes = chunks * q4_chunk_bytes(GPC);
     constexpr uint32_t CYCLE = 8 / GPC;  // chunks of eight groups
     const uint16_t* src[MT];
-    const uint8_t* rs[MT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-        src[i] = row(row0 + 16 * i);
-        if constexpr (!BIAS) rs[i] = sums(16 * i + (lane & 15)) + 16 * (lane >> 4);
-    }
+    for (int i = 0; i < MT; ++i) src[i] = row(row0 + 16 * i);
+    // the sums' 16-byte pieces, one a thread: row threadIdx / 4, piece threadIdx % 4 at 16 (4 row + (piece ^ (row / 4 & 3)))
+    const uint32_t srow = threadIdx.x >> 2, sto = 16 * (4 * srow + ((threadIdx.x & 3) ^ (srow >> 2 & 3)));
+    const uint8_t* rs = nullptr;
+    if constexpr (!BIAS) rs = sums(min(srow, 16u * MT - 1)) + 16 * (threadIdx.x & 3);
+    uint8_t* const lds_sums = lds + (RESIDENT ? terms * chunks : 2) * (MT * 4096);
     const uint32_t to = row0 * 256 + 16 * (piece ^ row0);  // row0 + 16 i: 4096 bytes further each
-    u4v ra[MT], rw[2][NT], rx[MT];
-    Q4Params<GPC> rp[2][NT];
+    u4v ra[MT], rw[AHEAD + 1][NT], rx{};
+    Q4Params<GPC> rp[AHEAD + 1][NT];
     Q4Biases<SBF, GPC> biases[NT];
+    struct Cursor {
+        uint32_t cb, term, c;
+    };
+    const auto next = [&](Cursor at) {
+        if (++at.c == chunks) at.c = 0, ++at.term;
+        if (at.term == terms) at.term = 0, at.cb += cb_step;
+        return at;
+    };
+    const auto inside = [&](const Cursor& at) { return at.cb * 4 * NT < tiles; };
     const auto load_rows = [&](uint32_t term, uint32_t c) {
         // past k, where the weights are zeros, the row's last 32 values again
         const uint32_t at = c * Q4_CHUNK + 8 * piece, off = at < k ? at : k - 32 + 8 * (piece & 3);
@@ -172,78 +185,115 @@ __device__ __forceinline__ void q4_gemm(uint8_t* lds, const uint8_t* w, uint32_t
 #pragma unroll
         for (int i = 0; i < MT; ++i) *reinterpret_cast<u4v*>(lds + buffer * (MT * 4096) + to + 4096 * i) = ra[i];
     };
-    const auto load = [&](int set, uint32_t cb_, uint32_t term, uint32_t c) {
+    const auto load = [&](int set, const Cursor& at) {
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            const uint32_t tile = min((cb_ * 4 + wave) * NT + t, tiles - 1);
-            const uint8_t* p = w + (size_t)tile * tile_bytes + (size_t)c * q4_chunk_bytes(GPC);
+            const uint32_t tile = min((at.cb * 4 + wave) * NT + t, tiles - 1);
+            const uint8_t* p = w + (size_t)tile * tile_bytes + (size_t)at.c * q4_chunk_bytes(GPC);
             rw[set][t] = reinterpret_cast<const u4v*>(p)[lane];
             rp[set][t] = q4_params<GPC>(p, lane);
         }
-        if constexpr (!RESIDENT) load_rows(term, c);
     };
     f4v out[NT][MT];
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) out[t][mt] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
-    uint32_t c = 0, term = 0;
+    Cursor at{cb, 0, 0}, far = at;  // the chunk that is multiplied, the one whose weights are read
+    uint32_t buffer = 0;
     // one chunk; false after the last
     const auto step = [&](auto set_) __attribute__((always_inline)) {
         constexpr int SET = decltype(set_)::value;
-        if constexpr (!RESIDENT) stage(SET);
+        const uint32_t c = at.c, term = at.term;
+        if constexpr (!RESIDENT) stage(buffer);
         const bool ends = c + 1 == chunks && term + 1 == terms;  // of the column block
-        uint32_t nc = c + 1, nterm = term, ncb = cb;
-        if (nc == chunks) nc = 0, ++nterm;
-        if (nterm == terms) nterm = 0, ncb += cb_step;
-        const bool more = ncb * 4 * NT < tiles;
-        if constexpr (!BIAS)
-            if (term == 0 && c % CYCLE == 0)
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) rx[mt] = *reinterpret_cast<const u4v*>(rs[mt] + c / CYCLE * 64);
-        if (more) load(1 - SET, ncb, nterm, nc);
+        const Cursor then = next(at);
+        const bool more = inside(then);
+        // Eight groups' sums are read with the first of their chunks, and go to LDS a chunk later (a barrier after the other
+        // buffer's last readers), or at once if no chunk follows: with one chunk in all, over the same values.
+        uint8_t* const cycle_sums = lds_sums + (c / CYCLE & 1) * (MT * 1024);
+        if constexpr (!BIAS && !RESIDENT)
+            if (term == 0) {
+                if (c % CYCLE == 0) rx = *reinterpret_cast<const u4v*>(rs + c / CYCLE * 64);
+                if ((c % CYCLE == 1 || (c % CYCLE == 0 && c + 1 == chunks)) && srow < 16u * MT)
+                    *reinterpret_cast<u4v*>(cycle_sums + sto) = rx;
+            }
+        if constexpr (!RESIDENT)
+            if (more) load_rows(then.term, then.c);
+        if (inside(far)) {
+            load((SET + AHEAD) % (AHEAD + 1), far);
+            far = next(far);
+        }
         if constexpr (!RESIDENT) __syncthreads();  // the chunk is staged; its buffer's last readers were before the last one
-        q4_gemm_chunk<BF, SBF, GPC, MT, NT, BIAS>(lds + (RESIDENT ? term * chunks + c : SET) * (MT * 4096), rw[SET], rp[SET],
+        q4_gemm_chunk<BF, SBF, GPC, MT, NT, BIAS>(lds + (RESIDENT ? term * chunks + c : buffer) * (MT * 4096), rw[SET], rp[SET],
                                                   lane, out);
         if constexpr (!BIAS)
             if (term == 0) {
 #pragma unroll
                 for (int t = 0; t < NT; ++t) biases[t].take(rp[SET][t]);
-                if (c % CYCLE == CYCLE - 1 || nc == 0) {
+                if (c % CYCLE == CYCLE - 1 || c + 1 == chunks) {
                     for (uint32_t i = c % CYCLE; i < CYCLE - 1; ++i) {  // no more chunks: zeros up to the eighth group
                         constexpr Q4Params<GPC> none{};
 #pragma unroll
                         for (int t = 0; t < NT; ++t) biases[t].take(none);
                     }
+                    u4v a[MT];
 #pragma unroll
-                    for (int t = 0; t < NT; ++t) biases[t].add(rx, out[t]);
+                    for (int mt = 0; mt < MT; ++mt) {
+                        const int r = mt * 16 + (lane & 15);
+                        a[mt] = *reinterpret_cast<const u4v*>(cycle_sums + 16 * (4 * r + ((lane >> 4) ^ (r >> 2 & 3))));
+                    }
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) biases[t].add(a, out[t]);
                 }
             }
         if (ends) {
+            // 16 rows of the wave's columns at a time, four columns a lane
+            float* const mine = reinterpret_cast<float*>(lds_sums + 2 * MT * 1024) + wave * q4_turn_floats<NT>();
+            const uint32_t tile0 = (at.cb * 4 + wave) * NT;
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const uint32_t tile = (cb * 4 + wave) * NT + t;
-                if (tile < tiles) store(tile, out[t]);
+            for (int mt = 0; mt < MT; ++mt) {
+                f4v v[NT];
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) out[t][mt] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+                for (int t = 0; t < NT; ++t) {
+                    v[t] = out[t][mt];
+                    out[t][mt] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+                }
+                q4_turn<NT>(mine, v, lane, [&](int r, int c, const f4v& p) {
+                    if (tile0 + c / 16 < tiles) store(16 * mt + r, tile0 * 16 + c, p);
+                });
             }
         }
-        c = nc;
-        term = nterm;
-        cb = ncb;
+        at = then;
+        buffer ^= 1;
         return more;
     };
-    load(0, cb, 0, 0);
+    if constexpr (!RESIDENT) load_rows(0, 0);
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+        if (inside(far)) {
+            load(i, far);
+            far = next(far);
+        }
     if constexpr (RESIDENT) {
         for (uint32_t t = 0; t < terms; ++t)
             for (uint32_t ci = 0; ci < chunks; ++ci) {
                 load_rows(t, ci);
                 stage(t * chunks + ci);
             }
+        if constexpr (!BIAS)
+            for (uint32_t i = 0; i * CYCLE < chunks; ++i)
+                if (srow < 16u * MT)
+                    *reinterpret_cast<u4v*>(lds_sums + i * (MT * 1024) + sto) = *reinterpret_cast<const u4v*>(rs + i * 64);
         __syncthreads();
     }
-    while (step(std::integral_constant<int, 0>{}) && step(std::integral_constant<int, 1>{})) {
-    }
+    if constexpr (AHEAD == 1)
+        while (step(std::integral_constant<int, 0>{}) && step(std::integral_constant<int, 1>{})) {
+        }
+    else
+        while (step(std::integral_constant<int, 0>{}) && step(std::integral_constant<int, 1>{}) &&
+               step(std::integral_constant<int, 2>{})) {
+        }
 }
 
 }  // namespace ea
