@@ -73,7 +73,11 @@ struct Q4LinArgs {
     int jobs;
 };
 
-// A block takes NT tiles of one job and 16 MT rows; its WK waves take every WK-th chunk and add their sums in wave order.
+// Up to 16 rows: a block takes NT tiles of one job and all rows; its WK waves take every WK-th chunk and add their sums in wave
+// order. Bound by the weights' bandwidth where there are many, by latencies where there are few; from then on by the rows,
+// which every block reads from L2, so wide jobs take four tiles a block, which share them: 65521 x 6144 at 1 / 8 / 16 rows
+// 41 / 46 / 54 us with four tiles (226 MB: 5.5 TB/s), 44 / 55 / 74 with two, 57 / 86 / 118 with one; but 8192 x 6144 at one row
+// 12.3, 9.9 and 9.4 us, where four tiles leave half of the card idle. 2048 x 6144: 5.4 us with 16 waves a tile.
 template <bool BF, bool SBF, int GPC, int MT, int NT, int WK, int NB>
 __global__ void __launch_bounds__(64 * WK) q4_linear_kernel(Q4LinArgs a) {
     __shared__ f4v part[WK][NT][MT][64];
@@ -106,29 +110,78 @@ __global__ void __launch_bounds__(64 * WK) q4_linear_kernel(Q4LinArgs a) {
     }
 }
 
-#ifndef LV
-#define LV 2
-#endif
-#ifndef LAH
-#define LAH 1
-#endif
-// More rows: 16 MT rows and 4 NT tiles a block.
-template <bool BF, bool SBF, int GPC, int MT, int NT>
-__global__ void __launch_bounds__(Q4_GEMM_THREADS, 2) q4_linear_gemm_kernel(Q4LinArgs a) {
-    __shared__ __attribute__((aligned(16))) uint8_t lds[q4_gemm_lds<MT, NT>()];
+// More rows: a block takes 16 MT rows and 4 NT tiles, and KS groups of four waves every KS-th chunk of them: each group stages
+// its chunk's rows in LDS, in two buffers, while the chunk before is multiplied, and reads its weights a chunk ahead; the
+// groups' sums are added in order at the end. Matrix and vector instructions hardly overlap here (measured: a product takes 17
+// cycles, a vector instruction 2.4 to 4.5, and together their sum), so waves count more than large tiles: 512 rows x 12000 x
+// 8192 take 189 us with 32 rows, two tiles and two groups, 198 with 64 rows, 212 without groups.
+template <bool BF, bool SBF, int GPC, int MT, int NT, int KS>
+__global__ void __launch_bounds__(256 * KS) q4_linear_split_kernel(Q4LinArgs a) {
+    constexpr int BUFFER = MT * 4096, PARTS = KS * 4 * NT * MT * 1024;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[2 * KS * BUFFER > PARTS ? 2 * KS * BUFFER : PARTS];
     const Q4Job job = a.job[blockIdx.z];
     const uint32_t tiles = q4_tiles(job.n), m0 = blockIdx.y * 16 * MT;
     if (blockIdx.x * 4 * NT >= tiles) return;
-    const int lane = threadIdx.x & 63;
-    q4_gemm<BF, SBF, GPC, MT, NT, true, false, LAH>(
-        lds, job.w, tiles, a.k, 1, 0, blockIdx.x, 1u << 24,
-        [&](uint32_t i) { return a.x + (size_t)min(m0 + i, a.m - 1) * a.x_stride; }, nullptr,
-        [&](uint32_t r, uint32_t n, const f4v& v) {
-            if (m0 + r >= a.m) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6 & 3);
+    const uint32_t group = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8), t256 = threadIdx.x & 255;
+    const uint32_t piece = t256 & 15, row0 = t256 >> 4, to = row0 * 256 + 16 * (piece ^ row0);
+    uint8_t* const mine = lds + group * 2 * BUFFER;
+    const uint8_t* w[NT];
+    const uint16_t* src[MT];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (n + i < job.n) store_act(job.y, job.y_dtype, (size_t)(m0 + r) * job.n + n + i, v[i]);
-        });
+    for (int t = 0; t < NT; ++t)
+        w[t] = job.w + (size_t)min((blockIdx.x * 4 + wave) * NT + t, tiles - 1) * a.chunks * q4_chunk_bytes(GPC);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) src[i] = a.x + (size_t)min(m0 + row0 + 16 * i, a.m - 1) * a.x_stride;
+    u4v ra[MT], rw[2][NT];
+    Q4Params<GPC> rp[2][NT];
+    const auto load = [&](int set, uint32_t c) {
+        c = min(c, a.chunks - 1);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const uint8_t* p = w[t] + (size_t)c * q4_chunk_bytes(GPC);
+            rw[set][t] = reinterpret_cast<const u4v*>(p)[lane];
+            rp[set][t] = q4_params<GPC>(p, lane);
+        }
+        const uint32_t at = c * Q4_CHUNK + 8 * piece, off = at < a.k ? at : a.k - 32 + 8 * (piece & 3);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) ra[i] = *reinterpret_cast<const u4v_a8*>(src[i] + off);
+    };
+    f4v out[NT][MT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) out[t][mt] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+    const auto step = [&](auto set_, uint32_t c) __attribute__((always_inline)) {  // every group takes every step
+        constexpr int SET = decltype(set_)::value;
+#pragma unroll
+        for (int i = 0; i < MT; ++i) *reinterpret_cast<u4v*>(mine + SET * BUFFER + to + 4096 * i) = ra[i];
+        load(1 - SET, c + KS);
+        __syncthreads();
+        if (c < a.chunks) q4_gemm_chunk<BF, SBF, GPC, MT, NT, true>(mine + SET * BUFFER, rw[SET], rp[SET], lane, out);
+    };
+    load(0, group);
+    for (uint32_t c0 = 0; c0 < a.chunks; c0 += 2 * KS) {
+        step(std::integral_constant<int, 0>{}, c0 + group);
+        if (c0 + KS < a.chunks) step(std::integral_constant<int, 1>{}, c0 + KS + group);
+    }
+    __syncthreads();
+    f4v(*part)[4][NT][MT][64] = reinterpret_cast<f4v(*)[4][NT][MT][64]>(lds);
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) part[group][wave][t][mt][lane] = out[t][mt];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 4 * NT * MT * 256; i += 256 * KS) {
+        const int n = i & 15, t = (i >> 4) % (4 * NT), r = (i / (64 * NT)) & 15, mt = i / (1024 * NT);
+        const uint32_t mr = m0 + 16 * mt + r, nc = (blockIdx.x * 4 * NT + t) * 16 + n;
+        if (mr >= a.m || nc >= job.n) continue;
+        const float* p = reinterpret_cast<const float*>(lds) + ((t * MT + mt) * 64 + (r >> 2) * 16 + n) * 4 + (r & 3);
+        float v = p[0];
+#pragma unroll
+        for (int g = 1; g < KS; ++g) v = v + p[g * 4 * NT * MT * 256];
+        store_act(job.y, job.y_dtype, (size_t)mr * job.n + nc, v);
+    }
 }
 
 static int launch_linear(hipStream_t s, const Q4LinArgs& a, uint32_t tiles, bool bf, bool sbf, int gpc) {
@@ -136,14 +189,16 @@ static int launch_linear(hipStream_t s, const Q4LinArgs& a, uint32_t tiles, bool
         constexpr int GPC = decltype(gpc_)::value;
         constexpr bool BF = decltype(bf_)::value, SBF = decltype(sbf_)::value;
         const unsigned jobs = (unsigned)a.jobs;
+        const auto blocks = [&](uint32_t rows, uint32_t nt) { return dim3((tiles + 4 * nt - 1) / (4 * nt), (a.m + rows - 1) / rows, jobs); };
         if (a.m <= 16) {
             if (tiles * jobs < 512) q4_linear_kernel<BF, SBF, GPC, 1, 1, 16, 3><<<dim3(tiles, 1, jobs), 1024, 0, s>>>(a);
-            else q4_linear_kernel<BF, SBF, GPC, 1, 2, 8, 3><<<dim3((tiles + 1) / 2, 1, jobs), 512, 0, s>>>(a);
-        } else {
-
-            if (LV == 0) q4_linear_kernel<BF, SBF, GPC, 4, 1, 8, 1><<<dim3(tiles, (a.m + 63) / 64, jobs), 512, 0, s>>>(a);
-            else q4_linear_gemm_kernel<BF, SBF, GPC, 4, LV ? LV : 1><<<dim3((tiles + 4 * LV - 1) / (4 * (LV ? LV : 1)), (a.m + 63) / 64, jobs), Q4_GEMM_THREADS, 0, s>>>(a);
+            else if (tiles * jobs < 1536) q4_linear_kernel<BF, SBF, GPC, 1, 2, 8, 3><<<dim3((tiles + 1) / 2, 1, jobs), 512, 0, s>>>(a);
+            else q4_linear_kernel<BF, SBF, GPC, 1, 4, 8, 2><<<dim3((tiles + 3) / 4, 1, jobs), 512, 0, s>>>(a);
+            return;
         }
+        const dim3 one = blocks(32, 1);
+        if (one.x * one.y * jobs <= 256) q4_linear_split_kernel<BF, SBF, GPC, 2, 1, 4><<<one, 1024, 0, s>>>(a);
+        else q4_linear_split_kernel<BF, SBF, GPC, 2, 2, 2><<<blocks(32, 2), 512, 0, s>>>(a);
     };
     q4_types(bf, sbf, gpc, go);
     return launched();

@@ -199,20 +199,6 @@ __device__ __forceinline__ void store_terms(uint16_t* h, int terms, size_t plane
     }
 }
 
-// Four neighbouring ones.
-__device__ __forceinline__ void store_terms4(uint16_t* h, int terms, size_t plane, size_t at, f4v v) {
-    for (int i = 0; i < terms; ++i) {
-        uint16_t b[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            b[k] = f2bf(v[k]);
-            v[k] = __builtin_fabsf(v[k]) < __builtin_inff() ? v[k] - bf2f(b[k]) : 0.0f;
-        }
-        *reinterpret_cast<u2v*>(h + (size_t)i * plane + at) =
-            u2v{(uint32_t)b[0] | (uint32_t)b[1] << 16, (uint32_t)b[2] | (uint32_t)b[3] << 16};
-    }
-}
-
 // ---- gate | up ------------------------------------------------------------------------------------------------------
 // Block (NT tiles of gate | up, item): 16 rows of a matrix instruction, those that the item does not have as zeros, which
 // cost neither loads nor cache; WK waves take every WK-th chunk. Up to 16 rows nothing is sorted before: block (tiles, pair)
@@ -427,14 +413,16 @@ __global__ void __launch_bounds__(256) q4_hsums_kernel(Q4MoeArgs a) {
 #define DAH 1
 #endif
 // ---- long items -----------------------------------------------------------------------------------------------------
-// An item's products by q4_gemm, with as many row groups as it has.
-template <bool BF, bool SBF, int GPC, int NT, bool RESIDENT, int AHEAD, typename ROW, typename SUMS, typename STORE>
+// An item's products by q4_gemm, with as many row groups as it has: NT4 tiles a wave with four of them, NT with fewer, whose
+// weights are read AHEAD chunks before. Column blocks are counted in 4 NT4 tiles; the ones behind the last return.
+template <bool BF, bool SBF, int GPC, int NT4, int NT, bool RESIDENT, bool TURN, int AHEAD, typename ROW, typename SUMS, typename STORE>
 __device__ __forceinline__ void q4_item_gemm(uint8_t* lds, int count, const uint8_t* w, uint32_t tiles, uint32_t k,
                                              uint32_t terms, size_t plane, uint32_t cb, uint32_t cb_step, ROW row,
                                              SUMS sums, STORE store) {
-    if (count <= 16) q4_gemm<BF, SBF, GPC, 1, NT, false, RESIDENT, AHEAD>(lds, w, tiles, k, terms, plane, cb, cb_step, row, sums, store);
-    else if (count <= 32) q4_gemm<BF, SBF, GPC, 2, NT, false, RESIDENT, AHEAD>(lds, w, tiles, k, terms, plane, cb, cb_step, row, sums, store);
-    else q4_gemm<BF, SBF, GPC, 4, NT, false, RESIDENT, AHEAD>(lds, w, tiles, k, terms, plane, cb, cb_step, row, sums, store);
+    if (count > 32) q4_gemm<BF, SBF, GPC, 4, NT4, false, RESIDENT, TURN, 1>(lds, w, tiles, k, terms, plane, cb, cb_step, row, sums, store);
+    else if (cb * 4 * NT >= tiles) return;
+    else if (count > 16) q4_gemm<BF, SBF, GPC, 2, NT, false, RESIDENT, TURN, AHEAD>(lds, w, tiles, k, terms, plane, cb, cb_step, row, sums, store);
+    else q4_gemm<BF, SBF, GPC, 1, NT, false, RESIDENT, TURN, AHEAD>(lds, w, tiles, k, terms, plane, cb, cb_step, row, sums, store);
 }
 
 // Blocks go to the card's eight dies in turn, and each die has an L2 of its own: die x takes the x-th eighth of the full items
@@ -448,35 +436,40 @@ constexpr int Q4_DIES = 8;
 __device__ __forceinline__ Q4Place q4_place(const Q4MoeArgs& a, uint32_t blocks) {
     const int n = a.nitems[0], full = a.nitems[1], rest = n - full;
     const int x = (int)(blockIdx.x % Q4_DIES);
-    const uint32_t slot = blockIdx.x / Q4_DIES, j = slot / blocks;
+    const uint32_t slot = blockIdx.x / Q4_DIES, each = gridDim.x / Q4_DIES / blocks, cb = slot / each;
+    const int j = (int)(slot - cb * each);
     const int f0 = (int)((int64_t)full * x / Q4_DIES), f1 = (int)((int64_t)full * (x + 1) / Q4_DIES);
     const int r0 = (int)((int64_t)rest * x / Q4_DIES), r1 = (int)((int64_t)rest * (x + 1) / Q4_DIES);
-    const int i = (int)j < f1 - f0 ? f0 + (int)j : full + r0 + (int)j - (f1 - f0);
-    return {i < (((int)j < f1 - f0) ? f1 : full + r1) ? i : -1, slot - j * blocks};
+    if (j < f1 - f0) return {f0 + j, cb};
+    const int i = full + r0 + j - (f1 - f0);
+    return {i < full + r1 ? i : -1, cb};
 }
 static unsigned q4_place_blocks(uint32_t max_items, uint32_t blocks) { return Q4_DIES * (max_items / Q4_DIES + 2) * blocks; }
 
-template <bool BF, bool SBF, int GPC, int NT>
+template <bool BF, bool SBF, int GPC, int NT4, int NT>
 __global__ void __launch_bounds__(Q4_GEMM_THREADS, WPS) q4_gateup_gemm_kernel(Q4MoeArgs a, uint32_t blocks) {
-    __shared__ __attribute__((aligned(16))) uint8_t lds[q4_gemm_lds<4, NT>()];
+    __shared__ __attribute__((aligned(16))) uint8_t lds[std::max(q4_gemm_lds<4, NT4>(), q4_gemm_lds<2, NT>())];
     const Q4Place at = q4_place(a, blocks);
     if (at.item < 0) return;
     const Q4Item& it = a.items[at.item];
     const int e = it.expert, count = it.count;
-    q4_item_gemm<BF, SBF, GPC, NT, false, GAH>(
+    q4_item_gemm<BF, SBF, GPC, NT4, NT, false, false, GAH>(
         lds, count, a.gu + (size_t)e * a.gu_bytes, (a.width + 7) / 8, a.dims, 1, 0, at.cb, 1u << 24,
         [&](int i) { return a.x + (size_t)((uint32_t)it.pair[min(i, count - 1)] / a.slots) * a.x_stride; },
         [&](int i) { return a.xsums + (size_t)((uint32_t)it.pair[min(i, count - 1)] / a.slots) * q4_sum_bytes(a.dims / a.group); },
-        [&](int m, uint32_t c, const f4v& v) {  // columns 0 .. 7 of 16 are the gate's, the others the up projection's
-            const uint32_t col = c / 16 * 8 + c % 8;
-            f4v u;
+        [&](uint32_t tile, const auto& v) {
+            const int lane = threadIdx.x & 63;
+            const uint32_t col = tile * 8 + (lane & 7);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) u[i] = lane_xor<2>(v[i]);
-            if ((c & 8) || m >= count || col >= a.width) return;
-            f4v h;
+            for (int mt = 0; mt < (int)(sizeof(v) / sizeof(f4v)); ++mt)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) h[i] = swiglu(v[i], u[i]);
-            store_terms4(a.h, a.terms, (size_t)a.pairs * a.width, (size_t)it.pair[m] * a.width + col, h);
+                for (int i = 0; i < 4; ++i) {
+                    const float u = lane_xor<8>(v[mt][i]);  // lanes 0 .. 7 of 16 have the gate, the others the up column
+                    const int m = 16 * mt + 4 * (lane >> 4) + i;
+                    if ((lane & 8) || m >= count || col >= a.width) continue;
+                    store_terms(a.h, a.terms, (size_t)a.pairs * a.width, (size_t)it.pair[m] * a.width + col,
+                                swiglu(v[mt][i], u));
+                }
         });
 }
 
@@ -487,7 +480,7 @@ __global__ void __launch_bounds__(Q4_GEMM_THREADS, WPS) q4_down_gemm_kernel(Q4Mo
     if (at.item < 0) return;
     const Q4Item& it = a.items[at.item];
     const int e = it.expert, count = it.count;
-    q4_item_gemm<true, SBF, GPC, NT, RESIDENT, DAH>(
+    q4_item_gemm<true, SBF, GPC, NT, NT, RESIDENT, true, DAH>(
         lds, count, a.down + (size_t)e * a.down_bytes, q4_tiles(a.dims), a.width, a.terms, (size_t)a.pairs * a.width,
         at.cb, blocks, [&](int i) { return a.h + (size_t)it.pair[min(i, count - 1)] * a.width; },
         [&](int i) { return a.hsums + (size_t)it.pair[min(i, count - 1)] * q4_sum_bytes(a.width / a.group); },
@@ -557,12 +550,13 @@ static void launch_gateup(hipStream_t s, const Q4MoeArgs& a, bool bf, bool sbf, 
         else if (a.rows <= 4 || (a.rows <= Q4_ROWS && tiles < 2)) q4_gateup_kernel<BF, SBF, GPC, 1, 8, 3, FEW_ROWS><<<one, 512, 0, s>>>(a);
         else if (a.rows <= Q4_ROWS) q4_gateup_kernel<BF, SBF, GPC, 2, 8, 3, FEW_ROWS><<<two, 512, 0, s>>>(a);
 #ifndef GNT
-#define GNT 4
+#define GNT 2
+#define GNT1 4
 #define DNT2 4
 #define DSP 6
 #endif
         else if (a.item == Q4_BIG_ITEM)
-            q4_gateup_gemm_kernel<BF, SBF, GPC, GNT><<<q4_place_blocks(max_items, (tiles + 4 * GNT - 1) / (4 * GNT)), Q4_GEMM_THREADS, 0, s>>>(a, (tiles + 4 * GNT - 1) / (4 * GNT));
+            q4_gateup_gemm_kernel<BF, SBF, GPC, GNT, GNT1><<<q4_place_blocks(max_items, (tiles + 4 * GNT - 1) / (4 * GNT)), Q4_GEMM_THREADS, 0, s>>>(a, (tiles + 4 * GNT - 1) / (4 * GNT));
         else if (tiles < 2) q4_gateup_kernel<BF, SBF, GPC, 1, 8, 3, ITEMS><<<dim3(1, max_items), 512, 0, s>>>(a);
         else q4_gateup_kernel<BF, SBF, GPC, 2, 8, 3, ITEMS><<<dim3((tiles + 1) / 2, max_items), 512, 0, s>>>(a);
     });
@@ -696,14 +690,16 @@ int ea_q4_routed(ea_stream_t stream, const void* x, int x_dtype, uint32_t x_stri
     a.slots = sc->slots;
     a.out_dtype = out_dtype;
     a.terms = q4_terms(out_dtype);
-    #ifndef BIGR
-#define BIGR 128
+        // Long items pay where experts have several rows each and there are blocks enough for a row of chunks apiece.
+#ifndef BIGR
+#define BIGR 512
 #endif
-    a.item = R > BIGR ? Q4_BIG_ITEM : Q4_ITEM;
+    const uint64_t some = std::min<uint64_t>(a.pairs, a.experts), column_blocks = ((a.width + 7) / 8 + 7) / 8;
+    const bool big = R > Q4_ROWS && a.pairs > 10 * some && (a.pairs / Q4_BIG_ITEM + some / 2) * column_blocks >= BIGR;
+    a.item = big ? Q4_BIG_ITEM : Q4_ITEM;
     const uint32_t max_items = q4_max_items(a.experts, a.pairs, a.item);
     hipStream_t s = as_stream(stream);
     const bool sbf = ex->s_dtype == BF16;
-    const bool big = a.item == Q4_BIG_ITEM;
     if (R > Q4_ROWS) q4_group_kernel<<<1 + (big ? (R + 15) / 16 : 0), 1024, 0, s>>>(a);
     launch_gateup(s, a, x_dtype == BF16, sbf, gpc, max_items);
     if (big) q4_hsums_kernel<<<(a.pairs + 3) / 4, 256, 0, s>>>(a);

@@ -10,9 +10,12 @@ namespace ea {
 
 constexpr int Q4_GEMM_THREADS = 256;
 // LDS: `buffers` chunks of 16 MT rows, 4096 MT bytes each, two buffers of their sums over eight groups, 1024 MT each, and the
-// waves' places to turn their sums.
+// waves' places to turn their sums: behind them (RESIDENT), or in the place of all.
 template <int MT, int NT>
-constexpr int q4_gemm_lds(int buffers = 2) { return buffers * MT * 4096 + 2 * MT * 1024 + 4 * 4 * q4_turn_floats<NT>(); }
+constexpr int q4_gemm_lds(int buffers = 0) {
+    const int turn = 4 * 4 * q4_turn_floats<NT>(), two = 2 * MT * (4096 + 1024);
+    return buffers ? buffers * MT * 4096 + 2 * MT * 1024 + turn : two > turn ? two : turn;
+}
 constexpr int Q4_RESIDENT = 4;  // chunks of all terms that stay in LDS at most
 
 // One chunk from LDS: row r of the block at 256 r, its 16-byte piece q at 16 (q ^ (r & 15)), so that the 16 rows of an
@@ -144,10 +147,10 @@ __device__ __forceinline__ void q4_row_sums(const uint16_t* row, uint32_t terms,
 
 // The column blocks cb, cb + cb_step, .. of W (its first tile at w) times the block's rows. row(i): row i's activations,
 // terms of them `plane` values apart (their products add up); sums(i): its groups' sums, for the biases, or with BIAS null.
-// store(row, column of W's packed rows, the sums of four columns). RESIDENT: all of the rows' terms and chunks lie in LDS at once (Q4_RESIDENT of
+// With TURN store(row, column of W's packed rows, the sums of four columns), else store(tile, the lane's sums). RESIDENT: all of the rows' terms and chunks lie in LDS at once (Q4_RESIDENT of
 // them at most), so that after the first barrier the waves go on alone; else two chunks do. Weights are read AHEAD (1 or
 // 2) chunks before their products.
-template <bool BF, bool SBF, int GPC, int MT, int NT, bool BIAS, bool RESIDENT, int AHEAD, typename ROW, typename SUMS, typename STORE>
+template <bool BF, bool SBF, int GPC, int MT, int NT, bool BIAS, bool RESIDENT, bool TURN, int AHEAD, typename ROW, typename SUMS, typename STORE>
 __device__ __forceinline__ void q4_gemm(uint8_t* lds, const uint8_t* w, uint32_t tiles, uint32_t k, uint32_t terms,
                                         size_t plane, uint32_t cb, uint32_t cb_step, ROW row, SUMS sums, STORE store) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -248,21 +251,30 @@ __device__ __forceinline__ void q4_gemm(uint8_t* lds, const uint8_t* w, uint32_t
                 }
             }
         if (ends) {
-            // 16 rows of the wave's columns at a time, four columns a lane
-            float* const mine = reinterpret_cast<float*>(lds_sums + 2 * MT * 1024) + wave * q4_turn_floats<NT>();
             const uint32_t tile0 = (at.cb * 4 + wave) * NT;
+            if constexpr (TURN) {  // 16 rows of the wave's columns at a time, where the chunks were once no wave reads them
+                if constexpr (!RESIDENT) __syncthreads();
+                float* const mine = reinterpret_cast<float*>(RESIDENT ? lds_sums + 2 * MT * 1024 : lds) + wave * q4_turn_floats<NT>();
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                f4v v[NT];
+                for (int mt = 0; mt < MT; ++mt) {
+                    f4v v[NT];
 #pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    v[t] = out[t][mt];
-                    out[t][mt] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+                    for (int t = 0; t < NT; ++t) v[t] = out[t][mt];
+                    q4_turn<NT>(mine, v, lane, [&](int r, int c, const f4v& p) {
+                        if (tile0 + c / 16 < tiles) store(16 * mt + r, tile0 * 16 + c, p);
+                    });
                 }
-                q4_turn<NT>(mine, v, lane, [&](int r, int c, const f4v& p) {
-                    if (tile0 + c / 16 < tiles) store(16 * mt + r, tile0 * 16 + c, p);
-                });
+                if constexpr (!RESIDENT)
+                    if (more) __syncthreads();
+            } else {
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+                    if (tile0 + t < tiles) store(tile0 + t, out[t]);
             }
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) out[t][mt] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
         }
         at = then;
         buffer ^= 1;
