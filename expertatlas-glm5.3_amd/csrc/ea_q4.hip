@@ -78,35 +78,27 @@ struct Q4LinArgs {
 // which every block reads from L2, so wide jobs take four tiles a block, which share them: 65521 x 6144 at 1 / 8 / 16 rows
 // 41 / 46 / 54 us with four tiles (226 MB: 5.5 TB/s), 44 / 55 / 74 with two, 57 / 86 / 118 with one; but 8192 x 6144 at one row
 // 12.3, 9.9 and 9.4 us, where four tiles leave half of the card idle. 2048 x 6144: 5.4 us with 16 waves a tile.
-template <bool BF, bool SBF, int GPC, int MT, int NT, int WK, int NB>
+template <bool BF, bool SBF, int GPC, int NT, int WK, int NB>
 __global__ void __launch_bounds__(64 * WK) q4_linear_kernel(Q4LinArgs a) {
-    __shared__ f4v part[WK][NT][MT][64];
+    __shared__ f4v part[WK][NT][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Q4Job job = a.job[blockIdx.z];
-    const uint32_t tiles = q4_tiles(job.n), tile0 = blockIdx.x * NT, m0 = blockIdx.y * 16 * MT;
+    const uint32_t tiles = q4_tiles(job.n), tile0 = blockIdx.x * NT;
     if (tile0 >= tiles) return;
     const size_t tile_bytes = (size_t)a.chunks * q4_chunk_bytes(GPC);
-    const uint32_t first = NT > 1 ? min(tile0, tiles - min(tiles, (uint32_t)NT)) : tile0;  // the last block's tiles overlap
-    const uint16_t* row[MT];
-    f4v out[NT][MT];
+    const uint32_t first = min(tile0, tiles - min(tiles, (uint32_t)NT));  // the last block's tiles overlap
+    const uint16_t* row = a.x + (size_t)min((uint32_t)(lane & 15), a.m - 1) * a.x_stride;  // rows past m re-read the last
+    f4v out[NT];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-        row[mt] = a.x + (size_t)min(m0 + 16 * mt + (lane & 15), a.m - 1) * a.x_stride;  // rows past m re-read the last
+    for (int t = 0; t < NT; ++t) out[t] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+    q4_stream<BF, SBF, GPC, NT, NB>(job.w + first * tile_bytes, tiles < NT ? 0 : tile_bytes, wave, WK, a.chunks, row, a.k, lane,
+                                    out);
 #pragma unroll
-        for (int t = 0; t < NT; ++t) out[t][mt] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
-    }
-    q4_stream<BF, SBF, GPC, MT, NT, NB>(job.w + first * tile_bytes, tiles < NT ? 0 : tile_bytes, wave, WK, a.chunks, row, a.k, lane,
-                                   out);
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) part[wave][t][mt][lane] = out[t][mt];
+    for (int t = 0; t < NT; ++t) part[wave][t][lane] = out[t];
     __syncthreads();
-    for (int i = threadIdx.x; i < 256 * MT * NT; i += 64 * WK) {
-        const int n = i & 15, t = (i >> 4) % NT, r = (i / (16 * NT)) & 15, mt = i / (256 * NT);
-        const uint32_t mr = m0 + 16 * mt + r, nc = (first + t) * 16 + n;
-        if (mr < a.m && nc < job.n && (NT == 1 || first + t < tiles))
-            store_act(job.y, job.y_dtype, (size_t)mr * job.n + nc, q4_total<WK, NT, MT>(part, t, mt, r, n));
+    for (uint32_t i = threadIdx.x; i < 16 * NT * a.m; i += 64 * WK) {
+        const uint32_t n = i & 15, t = (i >> 4) % NT, r = i / (16 * NT), col = (first + t) * 16 + n;
+        if (col < job.n) store_act(job.y, job.y_dtype, (size_t)r * job.n + col, q4_total<WK, NT>(part, t, r, n));
     }
 }
 
@@ -191,9 +183,9 @@ static int launch_linear(hipStream_t s, const Q4LinArgs& a, uint32_t tiles, bool
         const unsigned jobs = (unsigned)a.jobs;
         const auto blocks = [&](uint32_t rows, uint32_t nt) { return dim3((tiles + 4 * nt - 1) / (4 * nt), (a.m + rows - 1) / rows, jobs); };
         if (a.m <= 16) {
-            if (tiles * jobs < 512) q4_linear_kernel<BF, SBF, GPC, 1, 1, 16, 3><<<dim3(tiles, 1, jobs), 1024, 0, s>>>(a);
-            else if (tiles * jobs < 1536) q4_linear_kernel<BF, SBF, GPC, 1, 2, 8, 3><<<dim3((tiles + 1) / 2, 1, jobs), 512, 0, s>>>(a);
-            else q4_linear_kernel<BF, SBF, GPC, 1, 4, 8, 2><<<dim3((tiles + 3) / 4, 1, jobs), 512, 0, s>>>(a);
+            if (tiles * jobs < 512) q4_linear_kernel<BF, SBF, GPC, 1, 16, 3><<<dim3(tiles, 1, jobs), 1024, 0, s>>>(a);
+            else if (tiles * jobs < 1536) q4_linear_kernel<BF, SBF, GPC, 2, 8, 3><<<dim3((tiles + 1) / 2, 1, jobs), 512, 0, s>>>(a);
+            else q4_linear_kernel<BF, SBF, GPC, 4, 8, 2><<<dim3((tiles + 3) / 4, 1, jobs), 512, 0, s>>>(a);
             return;
         }
         const dim3 one = blocks(32, 1);

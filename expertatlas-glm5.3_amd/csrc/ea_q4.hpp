@@ -73,37 +73,28 @@ __device__ __forceinline__ void q4_scale_bias(uint32_t p, float& s, float& b) {
     b = SBF ? __builtin_bit_cast(float, p & 0xffff0000u) : h2f((uint16_t)(p >> 16));
 }
 
-// A chunk of NT tiles against MT groups of 16 rows: out += the chunk's share. a[mt][j]: the rows' A operands of the chunk's
-// four products. The sums of x come from the same operands against ones, which leaves them in the accumulators' own layout
-// (lane l: rows 4 (l >> 4) + i, weight row l & 15).
-template <bool BF, bool SBF, int GPC, int MT, int NT>
-__device__ __forceinline__ void q4_chunk(const u4v (&words)[NT], const Q4Params<GPC> (&par)[NT], const u4v (&a)[MT][4],
-                                         f4v (&out)[NT][MT]) {
+// A chunk of NT tiles against 16 rows: out += the chunk's share. a[j]: the rows' A operands of the chunk's four products. The
+// sums of x come from the same operands against ones, which leaves them in the accumulators' own layout (lane l: rows
+// 4 (l >> 4) + i, weight row l & 15).
+template <bool BF, bool SBF, int GPC, int NT>
+__device__ __forceinline__ void q4_chunk(const u4v (&words)[NT], const Q4Params<GPC> (&par)[NT], const u4v (&a)[4],
+                                         f4v (&out)[NT]) {
     constexpr int JPG = 4 / GPC;
     const f4v zero{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int g = 0; g < GPC; ++g) {
-        f4v xs[MT];
+        f4v xs;
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int j = 0; j < JPG; ++j) xs[mt] = q4_mfma<BF>(a[mt][g * JPG + j], q4_ones<BF>(), j ? xs[mt] : zero);
+        for (int j = 0; j < JPG; ++j) xs = q4_mfma<BF>(a[g * JPG + j], q4_ones<BF>(), j ? xs : zero);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            f4v acc[MT];
+            f4v acc;
 #pragma unroll
-            for (int j = 0; j < JPG; ++j) {
-                const u4v b = q4_values<BF>(words[t][g * JPG + j]);
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) acc[mt] = q4_mfma<BF>(a[mt][g * JPG + j], b, j ? acc[mt] : zero);
-            }
+            for (int j = 0; j < JPG; ++j) acc = q4_mfma<BF>(a[g * JPG + j], q4_values<BF>(words[t][g * JPG + j]), j ? acc : zero);
             float s, b;
             q4_scale_bias<SBF>(par[t].w[g], s, b);
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    out[t][mt][i] = __builtin_fmaf(b, xs[mt][i], __builtin_fmaf(s, acc[mt][i], out[t][mt][i]));
+            for (int i = 0; i < 4; ++i) out[t][i] = __builtin_fmaf(b, xs[i], __builtin_fmaf(s, acc[i], out[t][i]));
         }
     }
 }
@@ -117,14 +108,13 @@ __device__ __forceinline__ void q4_rows(const uint16_t* row, uint32_t chunk, uin
     for (int j = 0; j < 4; ++j) a[j] = (u4v) * reinterpret_cast<const u4v_a8*>(p + min(32 * j, last));
 }
 
-// The tiles at w, w + tile_bytes, .. against MT groups of 16 rows over the chunks c0, c0 + step, ..: the loads of NB chunks
-// are issued before the first of their products. With SOME, a lane whose row is null reads nothing and multiplies zeros.
-template <bool BF, bool SBF, int GPC, int MT, int NT, int NB, bool SOME = false>
+// The tiles at w, w + tile_bytes, .. against 16 rows over the chunks c0, c0 + step, ..: the loads of NB chunks are issued
+// before the first of their products. With SOME, a lane whose row is null reads nothing and multiplies zeros.
+template <bool BF, bool SBF, int GPC, int NT, int NB, bool SOME = false>
 __device__ __forceinline__ void q4_stream(const uint8_t* w, size_t tile_bytes, uint32_t c0, uint32_t step, uint32_t chunks,
-                                          const uint16_t* const (&row)[MT], uint32_t k, int lane,
-                                          f4v (&out)[NT][MT]) {
+                                          const uint16_t* row, uint32_t k, int lane, f4v (&out)[NT]) {
     for (uint32_t c = c0; c < chunks; c += step * NB) {
-        u4v words[NB][NT], x[NB][MT][4];
+        u4v words[NB][NT], x[NB][4];
         Q4Params<GPC> par[NB][NT];
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
@@ -135,35 +125,32 @@ __device__ __forceinline__ void q4_stream(const uint8_t* w, size_t tile_bytes, u
                 words[i][t] = reinterpret_cast<const u4v*>(p)[lane];
                 par[i][t] = q4_params<GPC>(p, lane);
             }
-            if constexpr (!SOME)
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) q4_rows(row[mt], ci, k, lane, x[i][mt]);
+            if constexpr (!SOME) q4_rows(row, ci, k, lane, x[i]);
         }
         if constexpr (SOME) {
-            static_assert(MT == 1, "one row a lane");
 #pragma unroll
             for (int i = 0; i < NB; ++i)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) x[i][0][j] = u4v{0, 0, 0, 0};
-            if (row[0]) {
+                for (int j = 0; j < 4; ++j) x[i][j] = u4v{0, 0, 0, 0};
+            if (row) {
 #pragma unroll
-                for (int i = 0; i < NB; ++i) q4_rows(row[0], min(c + step * i, chunks - 1), k, lane, x[i][0]);
+                for (int i = 0; i < NB; ++i) q4_rows(row, min(c + step * i, chunks - 1), k, lane, x[i]);
             }
         }
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < NB; ++i)
-            if (c + step * i < chunks) q4_chunk<BF, SBF, GPC, MT, NT>(words[i], par[i], x[i], out);
+            if (c + step * i < chunks) q4_chunk<BF, SBF, GPC, NT>(words[i], par[i], x[i], out);
     }
 }
 
-// Value (row r of group mt, weight row n of tile t) summed over the waves' parts, in wave order.
-template <int WK, int NT, int MT>
-__device__ __forceinline__ float q4_total(const f4v (&part)[WK][NT][MT][64], int t, int mt, int r, int n) {
-    const float* all = reinterpret_cast<const float*>(part) + ((t * MT + mt) * 64 + (r >> 2) * 16 + n) * 4 + (r & 3);
+// Value (row r, weight row n of tile t) summed over the waves' parts, in wave order.
+template <int WK, int NT>
+__device__ __forceinline__ float q4_total(const f4v (&part)[WK][NT][64], int t, int r, int n) {
+    const float* all = reinterpret_cast<const float*>(part) + (t * 64 + (r >> 2) * 16 + n) * 4 + (r & 3);
     float v = all[0];
 #pragma unroll
-    for (int k = 1; k < WK; ++k) v = v + all[k * NT * MT * 256];
+    for (int k = 1; k < WK; ++k) v = v + all[k * NT * 256];
     return v;
 }
 

@@ -50,7 +50,7 @@ struct Q4MoeArgs {
 __device__ void q4_group(const Q4MoeArgs& a) {
     __shared__ uint32_t count[Q4_MAX_EXPERTS], full[Q4_MAX_EXPERTS], rest[Q4_MAX_EXPERTS], sums[2][16], all;
     __shared__ uint16_t nfull[Q4_MAX_EXPERTS];  // at most EA_Q4_MAX_PAIRS / Q4_ITEM
-    constexpr int KEEP = 8;  // picks a thread keeps between the passes
+    constexpr int KEEP = 16;  // picks a thread keeps between the passes
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     uint32_t kept[KEEP];
 #pragma unroll
@@ -208,17 +208,17 @@ enum Q4Rows { ONE_ROW, FEW_ROWS, ITEMS };
 
 template <bool BF, bool SBF, int GPC, int NT, int WK, int NB, int MODE>
 __global__ void __launch_bounds__(64 * WK) q4_gateup_kernel(Q4MoeArgs a) {
-    __shared__ f4v part[WK][NT][1][64];
+    __shared__ f4v part[WK][NT][64];
     __shared__ int32_t picks[MODE == FEW_ROWS ? Q4_PAIRS : 16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t u = blockIdx.y, chunks = q4_chunks(a.dims), tiles = (a.width + 7) / 8, r = lane & 15;
     int32_t e;
-    const uint16_t* row[1] = {nullptr};
+    const uint16_t* row = nullptr;
     int count = 0;
     if constexpr (MODE == ONE_ROW) {  // every slot by itself: nothing is compared before the weights are read
         e = a.pick[u];
         if ((uint32_t)e >= a.experts) return;
-        if (r == 0) row[0] = a.x;
+        if (r == 0) row = a.x;
     } else if constexpr (MODE == FEW_ROWS) {
         for (uint32_t p = threadIdx.x; p < a.pairs; p += 64 * WK) picks[p] = a.pick[p];
         __syncthreads();
@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(64 * WK) q4_gateup_kernel(Q4MoeArgs a) {
         if (__ballot(before)) return;
         if (r < a.rows)
             for (uint32_t k = 0; k < a.slots; ++k)
-                if (picks[r * a.slots + k] == e) row[0] = a.x + (size_t)r * a.x_stride;
+                if (picks[r * a.slots + k] == e) row = a.x + (size_t)r * a.x_stride;
     } else {
         const Q4Item& it = a.items[u];
         const int n = *a.nitems, p = it.pair[r];  // read together; what lies behind the items is not used
@@ -241,17 +241,17 @@ __global__ void __launch_bounds__(64 * WK) q4_gateup_kernel(Q4MoeArgs a) {
         count = it.count;
         if ((int)u >= n) return;
         if (threadIdx.x < 16) picks[r] = p;
-        if ((int)r < count) row[0] = a.x + (size_t)((uint32_t)p / a.slots) * a.x_stride;
+        if ((int)r < count) row = a.x + (size_t)((uint32_t)p / a.slots) * a.x_stride;
     }
     const uint32_t tile0 = min(blockIdx.x * NT, tiles - NT);  // the last block's tiles overlap
     const size_t tile_bytes = (size_t)chunks * q4_chunk_bytes(GPC);
-    f4v out[NT][1];
+    f4v out[NT];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) out[t][0] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
-    q4_stream<BF, SBF, GPC, 1, NT, NB, true>(a.gu + (size_t)e * a.gu_bytes + tile0 * tile_bytes, tile_bytes, wave, WK, chunks, row,
+    for (int t = 0; t < NT; ++t) out[t] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+    q4_stream<BF, SBF, GPC, NT, NB, true>(a.gu + (size_t)e * a.gu_bytes + tile0 * tile_bytes, tile_bytes, wave, WK, chunks, row,
                                         a.dims, lane, out);
 #pragma unroll
-    for (int t = 0; t < NT; ++t) part[wave][t][0][lane] = out[t][0];
+    for (int t = 0; t < NT; ++t) part[wave][t][lane] = out[t];
     __syncthreads();
     for (int i = threadIdx.x; i < 128 * NT; i += 64 * WK) {
         const int n = i & 7, t = (i >> 3) % NT, m = i / (8 * NT);
@@ -270,7 +270,7 @@ __global__ void __launch_bounds__(64 * WK) q4_gateup_kernel(Q4MoeArgs a) {
             is = is && m < count;
         }
         if (!is) continue;
-        const float v = swiglu(q4_total<WK, NT, 1>(part, t, 0, m, n), q4_total<WK, NT, 1>(part, t, 0, m, n + 8));
+        const float v = swiglu(q4_total<WK, NT>(part, t, m, n), q4_total<WK, NT>(part, t, m, n + 8));
         store_terms(a.h, a.terms, (size_t)a.pairs * a.width, (size_t)p * a.width + col, v);
     }
 }
@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(64 * WK) q4_gateup_kernel(Q4MoeArgs a) {
 // terms (rows 0 .. TERMS - 1 of the instruction) and waves are added at the end.
 template <bool SBF, int GPC, int TERMS, int NT, int WK, int NB>
 __global__ void __launch_bounds__(64 * WK) q4_down_one_kernel(Q4MoeArgs a) {
-    __shared__ f4v part[WK][NT][1][64];
+    __shared__ f4v part[WK][NT][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), term = lane & 15;
     const uint32_t chunks = q4_chunks(a.width), tiles = q4_tiles(a.dims), units = a.slots * chunks;
     const uint32_t tile0 = min(blockIdx.x * NT, tiles - NT);
@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(64 * WK) q4_down_one_kernel(Q4MoeArgs a) {
 #pragma unroll
     for (int t = 0; t < NT; ++t) out[t] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
     for (uint32_t u0 = wave; u0 < units; u0 += WK * NB) {
-        u4v words[NB][NT], x[NB][1][4];
+        u4v words[NB][NT], x[NB][4];
         Q4Params<GPC> par[NB][NT];
         int32_t e[NB];
         float w[NB];
@@ -313,38 +313,38 @@ __global__ void __launch_bounds__(64 * WK) q4_down_one_kernel(Q4MoeArgs a) {
 #pragma unroll
         for (int i = 0; i < NB; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x[i][0][j] = u4v{0, 0, 0, 0};
+            for (int j = 0; j < 4; ++j) x[i][j] = u4v{0, 0, 0, 0};
         if (term < TERMS) {
 #pragma unroll
             for (int i = 0; i < NB; ++i) {
                 const uint32_t u = min(u0 + WK * i, units - 1);
-                q4_rows(a.h + term * plane + (size_t)(u / chunks) * a.width, u % chunks, a.width, lane, x[i][0]);
+                q4_rows(a.h + term * plane + (size_t)(u / chunks) * a.width, u % chunks, a.width, lane, x[i]);
             }
         }
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
             if (u0 + WK * i >= units || (uint32_t)e[i] >= a.experts) continue;
-            f4v y[NT][1];
+            f4v y[NT];
 #pragma unroll
-            for (int t = 0; t < NT; ++t) y[t][0] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
-            q4_chunk<true, SBF, GPC, 1, NT>(words[i], par[i], x[i], y);
+            for (int t = 0; t < NT; ++t) y[t] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+            q4_chunk<true, SBF, GPC, NT>(words[i], par[i], x[i], y);
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int r = 0; r < TERMS; ++r) out[t][r] = __builtin_fmaf(w[i], y[t][0][r], out[t][r]);
+                for (int r = 0; r < TERMS; ++r) out[t][r] = __builtin_fmaf(w[i], y[t][r], out[t][r]);
         }
     }
 #pragma unroll
-    for (int t = 0; t < NT; ++t) part[wave][t][0][lane] = out[t];
+    for (int t = 0; t < NT; ++t) part[wave][t][lane] = out[t];
     __syncthreads();
     for (int i = threadIdx.x; i < 16 * NT; i += 64 * WK) {
         const int n = i & 15, t = i >> 4;
         const uint32_t col = (tile0 + t) * 16 + n;
         if (col >= a.dims) continue;
-        float v = q4_total<WK, NT, 1>(part, t, 0, TERMS - 1, n);
+        float v = q4_total<WK, NT>(part, t, TERMS - 1, n);
 #pragma unroll
-        for (int r = TERMS - 2; r >= 0; --r) v = v + q4_total<WK, NT, 1>(part, t, 0, r, n);  // the small terms first
+        for (int r = TERMS - 2; r >= 0; --r) v = v + q4_total<WK, NT>(part, t, r, n);  // the small terms first
         store_act(a.out, a.out_dtype, col, v);
     }
 }
@@ -368,23 +368,23 @@ __global__ void __launch_bounds__(64 * WK) q4_down_kernel(Q4MoeArgs a) {
     const uint8_t* w = a.down + (size_t)e * a.down_bytes;
     const int term = (lane & 15) / PER;
     for (int m0 = 0; m0 < count; m0 += PER) {
-        const uint16_t* row[1] = {nullptr};
+        const uint16_t* row = nullptr;
         if (m0 + (lane & (PER - 1)) < count && term < TERMS)
-            row[0] = a.h + term * plane + (size_t)(m0 ? it.pair[m0 + (lane & (PER - 1))] : from) * a.width;
+            row = a.h + term * plane + (size_t)(m0 ? it.pair[m0 + (lane & (PER - 1))] : from) * a.width;
         const uint32_t mine = (blockIdx.x * WK + wave) * NT;
         if (mine < tiles) {
             const uint32_t tile0 = min(mine, tiles - NT);  // the last wave's tiles overlap
-            f4v out[NT][1];
+            f4v out[NT];
 #pragma unroll
-            for (int t = 0; t < NT; ++t) out[t][0] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
-            q4_stream<true, SBF, GPC, 1, NT, NB, true>(w + tile0 * tile_bytes, tile_bytes, 0, 1, chunks, row, a.width, lane,
+            for (int t = 0; t < NT; ++t) out[t] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+            q4_stream<true, SBF, GPC, NT, NB, true>(w + tile0 * tile_bytes, tile_bytes, 0, 1, chunks, row, a.width, lane,
                                                   out);
             f4v v[NT];
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    v[t][i] = out[t][0][i];
+                    v[t][i] = out[t][i];
                     if constexpr (TERMS == 3) v[t][i] = v[t][i] + lane_xor<16>(v[t][i]);
                     if constexpr (TERMS >= 2) v[t][i] = v[t][i] + lane_xor<32>(v[t][i]);
                 }
@@ -405,24 +405,17 @@ __global__ void __launch_bounds__(256) q4_hsums_kernel(Q4MoeArgs a) {
                           a.hsums + (size_t)i * q4_sum_bytes(a.width / a.group), threadIdx.x & 63);
 }
 
-#ifndef WPS
-#define WPS 2
-#endif
-#ifndef GAH
-#define GAH 1
-#define DAH 1
-#endif
 // ---- long items -----------------------------------------------------------------------------------------------------
-// An item's products by q4_gemm, with as many row groups as it has: NT4 tiles a wave with four of them, NT with fewer, whose
-// weights are read AHEAD chunks before. Column blocks are counted in 4 NT4 tiles; the ones behind the last return.
-template <bool BF, bool SBF, int GPC, int NT4, int NT, bool RESIDENT, bool TURN, int AHEAD, typename ROW, typename SUMS, typename STORE>
+// An item's products by q4_gemm, with as many row groups as it has: NT4 tiles a wave with four of them, NT with fewer.
+// Column blocks are counted in 4 NT4 tiles; the ones behind the last return.
+template <bool BF, bool SBF, int GPC, int NT4, int NT, bool RESIDENT, bool TURN, typename ROW, typename SUMS, typename STORE>
 __device__ __forceinline__ void q4_item_gemm(uint8_t* lds, int count, const uint8_t* w, uint32_t tiles, uint32_t k,
                                              uint32_t terms, size_t plane, uint32_t cb, uint32_t cb_step, ROW row,
                                              SUMS sums, STORE store) {
-    if (count > 32) q4_gemm<BF, SBF, GPC, 4, NT4, false, RESIDENT, TURN, 1>(lds, w, tiles, k, terms, plane, cb, cb_step, row, sums, store);
+    if (count > 32) q4_gemm<BF, SBF, GPC, 4, NT4, RESIDENT, TURN>(lds, w, tiles, k, terms, plane, cb, cb_step, row, sums, store);
     else if (cb * 4 * NT >= tiles) return;
-    else if (count > 16) q4_gemm<BF, SBF, GPC, 2, NT, false, RESIDENT, TURN, AHEAD>(lds, w, tiles, k, terms, plane, cb, cb_step, row, sums, store);
-    else q4_gemm<BF, SBF, GPC, 1, NT, false, RESIDENT, TURN, AHEAD>(lds, w, tiles, k, terms, plane, cb, cb_step, row, sums, store);
+    else if (count > 16) q4_gemm<BF, SBF, GPC, 2, NT, RESIDENT, TURN>(lds, w, tiles, k, terms, plane, cb, cb_step, row, sums, store);
+    else q4_gemm<BF, SBF, GPC, 1, NT, RESIDENT, TURN>(lds, w, tiles, k, terms, plane, cb, cb_step, row, sums, store);
 }
 
 // Blocks go to the card's eight dies in turn, and each die has an L2 of its own: die x takes the x-th eighth of the full items
@@ -447,13 +440,13 @@ __device__ __forceinline__ Q4Place q4_place(const Q4MoeArgs& a, uint32_t blocks)
 static unsigned q4_place_blocks(uint32_t max_items, uint32_t blocks) { return Q4_DIES * (max_items / Q4_DIES + 2) * blocks; }
 
 template <bool BF, bool SBF, int GPC, int NT4, int NT>
-__global__ void __launch_bounds__(Q4_GEMM_THREADS, WPS) q4_gateup_gemm_kernel(Q4MoeArgs a, uint32_t blocks) {
+__global__ void __launch_bounds__(Q4_GEMM_THREADS, 2) q4_gateup_gemm_kernel(Q4MoeArgs a, uint32_t blocks) {
     __shared__ __attribute__((aligned(16))) uint8_t lds[std::max(q4_gemm_lds<4, NT4>(), q4_gemm_lds<2, NT>())];
     const Q4Place at = q4_place(a, blocks);
     if (at.item < 0) return;
     const Q4Item& it = a.items[at.item];
     const int e = it.expert, count = it.count;
-    q4_item_gemm<BF, SBF, GPC, NT4, NT, false, false, GAH>(
+    q4_item_gemm<BF, SBF, GPC, NT4, NT, false, false>(
         lds, count, a.gu + (size_t)e * a.gu_bytes, (a.width + 7) / 8, a.dims, 1, 0, at.cb, 1u << 24,
         [&](int i) { return a.x + (size_t)((uint32_t)it.pair[min(i, count - 1)] / a.slots) * a.x_stride; },
         [&](int i) { return a.xsums + (size_t)((uint32_t)it.pair[min(i, count - 1)] / a.slots) * q4_sum_bytes(a.dims / a.group); },
@@ -474,13 +467,13 @@ __global__ void __launch_bounds__(Q4_GEMM_THREADS, WPS) q4_gateup_gemm_kernel(Q4
 }
 
 template <bool SBF, int GPC, int NT, bool RESIDENT>
-__global__ void __launch_bounds__(Q4_GEMM_THREADS, WPS) q4_down_gemm_kernel(Q4MoeArgs a, uint32_t blocks) {
+__global__ void __launch_bounds__(Q4_GEMM_THREADS, 2) q4_down_gemm_kernel(Q4MoeArgs a, uint32_t blocks) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const Q4Place at = q4_place(a, blocks);
     if (at.item < 0) return;
     const Q4Item& it = a.items[at.item];
     const int e = it.expert, count = it.count;
-    q4_item_gemm<true, SBF, GPC, NT, NT, RESIDENT, true, DAH>(
+    q4_item_gemm<true, SBF, GPC, NT, NT, RESIDENT, true>(
         lds, count, a.down + (size_t)e * a.down_bytes, q4_tiles(a.dims), a.width, a.terms, (size_t)a.pairs * a.width,
         at.cb, blocks, [&](int i) { return a.h + (size_t)it.pair[min(i, count - 1)] * a.width; },
         [&](int i) { return a.hsums + (size_t)it.pair[min(i, count - 1)] * q4_sum_bytes(a.width / a.group); },
@@ -549,14 +542,8 @@ static void launch_gateup(hipStream_t s, const Q4MoeArgs& a, bool bf, bool sbf, 
         if (a.rows == 1) q4_gateup_kernel<BF, SBF, GPC, 1, 8, 3, ONE_ROW><<<one, 512, 0, s>>>(a);
         else if (a.rows <= 4 || (a.rows <= Q4_ROWS && tiles < 2)) q4_gateup_kernel<BF, SBF, GPC, 1, 8, 3, FEW_ROWS><<<one, 512, 0, s>>>(a);
         else if (a.rows <= Q4_ROWS) q4_gateup_kernel<BF, SBF, GPC, 2, 8, 3, FEW_ROWS><<<two, 512, 0, s>>>(a);
-#ifndef GNT
-#define GNT 2
-#define GNT1 4
-#define DNT2 4
-#define DSP 6
-#endif
         else if (a.item == Q4_BIG_ITEM)
-            q4_gateup_gemm_kernel<BF, SBF, GPC, GNT, GNT1><<<q4_place_blocks(max_items, (tiles + 4 * GNT - 1) / (4 * GNT)), Q4_GEMM_THREADS, 0, s>>>(a, (tiles + 4 * GNT - 1) / (4 * GNT));
+            q4_gateup_gemm_kernel<BF, SBF, GPC, 2, 4><<<q4_place_blocks(max_items, (tiles + 7) / 8), Q4_GEMM_THREADS, 0, s>>>(a, (tiles + 7) / 8);
         else if (tiles < 2) q4_gateup_kernel<BF, SBF, GPC, 1, 8, 3, ITEMS><<<dim3(1, max_items), 512, 0, s>>>(a);
         else q4_gateup_kernel<BF, SBF, GPC, 2, 8, 3, ITEMS><<<dim3((tiles + 1) / 2, max_items), 512, 0, s>>>(a);
     });
@@ -572,12 +559,12 @@ static void launch_down(hipStream_t s, const Q4MoeArgs& a, bool sbf, int gpc, ui
             if (a.rows == 1) q4_down_one_kernel<SBF, GPC, TERMS, 1, 8, 2><<<tiles, 512, 0, s>>>(a);
             else if (a.item == Q4_BIG_ITEM)
                 [&] {
-                    const uint32_t blocks = std::min((tiles + 4 * DNT2 - 1) / (4 * DNT2), (uint32_t)DSP);
+                    const uint32_t blocks = std::min((tiles + 15) / 16, 6u);
                     const unsigned grid = q4_place_blocks(max_items, blocks);
                     const uint32_t buffers = TERMS * q4_chunks(a.width);
                     if (buffers <= Q4_RESIDENT)
-                        q4_down_gemm_kernel<SBF, GPC, DNT2, true><<<grid, Q4_GEMM_THREADS, q4_gemm_lds<4, DNT2>(buffers), s>>>(a, blocks);
-                    else q4_down_gemm_kernel<SBF, GPC, DNT2, false><<<grid, Q4_GEMM_THREADS, q4_gemm_lds<4, DNT2>(), s>>>(a, blocks);
+                        q4_down_gemm_kernel<SBF, GPC, 4, true><<<grid, Q4_GEMM_THREADS, q4_gemm_lds<4, 4>(buffers), s>>>(a, blocks);
+                    else q4_down_gemm_kernel<SBF, GPC, 4, false><<<grid, Q4_GEMM_THREADS, q4_gemm_lds<4, 4>(), s>>>(a, blocks);
                 }();
             else if (tiles >= 4) q4_down_kernel<SBF, GPC, TERMS, 4, 8, 1><<<dim3((tiles + 31) / 32, max_items), 512, 0, s>>>(a);
             else q4_down_kernel<SBF, GPC, TERMS, 1, 4, 1><<<dim3((tiles + 3) / 4, max_items), 256, 0, s>>>(a);
@@ -691,11 +678,8 @@ int ea_q4_routed(ea_stream_t stream, const void* x, int x_dtype, uint32_t x_stri
     a.out_dtype = out_dtype;
     a.terms = q4_terms(out_dtype);
         // Long items pay where experts have several rows each and there are blocks enough for a row of chunks apiece.
-#ifndef BIGR
-#define BIGR 512
-#endif
     const uint64_t some = std::min<uint64_t>(a.pairs, a.experts), column_blocks = ((a.width + 7) / 8 + 7) / 8;
-    const bool big = R > Q4_ROWS && a.pairs > 10 * some && (a.pairs / Q4_BIG_ITEM + some / 2) * column_blocks >= BIGR;
+    const bool big = R > Q4_ROWS && a.pairs > 10 * some && (a.pairs / Q4_BIG_ITEM + some / 2) * column_blocks >= 512;
     a.item = big ? Q4_BIG_ITEM : Q4_ITEM;
     const uint32_t max_items = q4_max_items(a.experts, a.pairs, a.item);
     hipStream_t s = as_stream(stream);

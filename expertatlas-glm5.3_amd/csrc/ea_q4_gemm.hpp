@@ -146,11 +146,11 @@ __device__ __forceinline__ void q4_row_sums(const uint16_t* row, uint32_t terms,
 }
 
 // The column blocks cb, cb + cb_step, .. of W (its first tile at w) times the block's rows. row(i): row i's activations,
-// terms of them `plane` values apart (their products add up); sums(i): its groups' sums, for the biases, or with BIAS null.
-// With TURN store(row, column of W's packed rows, the sums of four columns), else store(tile, the lane's sums). RESIDENT: all of the rows' terms and chunks lie in LDS at once (Q4_RESIDENT of
-// them at most), so that after the first barrier the waves go on alone; else two chunks do. Weights are read AHEAD (1 or
-// 2) chunks before their products.
-template <bool BF, bool SBF, int GPC, int MT, int NT, bool BIAS, bool RESIDENT, bool TURN, int AHEAD, typename ROW, typename SUMS, typename STORE>
+// terms of them `plane` values apart (their products add up); sums(i): its groups' sums, for the biases. With TURN store(row,
+// column of W's packed rows, the sums of four columns), else store(tile, the lane's sums). RESIDENT: all of the rows' terms and
+// chunks lie in LDS at once (Q4_RESIDENT of them at most), so that after the first barrier the waves go on alone; else two
+// chunks do. Weights are read a chunk before their products.
+template <bool BF, bool SBF, int GPC, int MT, int NT, bool RESIDENT, bool TURN, typename ROW, typename SUMS, typename STORE>
 __device__ __forceinline__ void q4_gemm(uint8_t* lds, const uint8_t* w, uint32_t tiles, uint32_t k, uint32_t terms,
                                         size_t plane, uint32_t cb, uint32_t cb_step, ROW row, SUMS sums, STORE store) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -162,12 +162,11 @@ __device__ __forceinline__ void q4_gemm(uint8_t* lds, const uint8_t* w, uint32_t
     for (int i = 0; i < MT; ++i) src[i] = row(row0 + 16 * i);
     // the sums' 16-byte pieces, one a thread: row threadIdx / 4, piece threadIdx % 4 at 16 (4 row + (piece ^ (row / 4 & 3)))
     const uint32_t srow = threadIdx.x >> 2, sto = 16 * (4 * srow + ((threadIdx.x & 3) ^ (srow >> 2 & 3)));
-    const uint8_t* rs = nullptr;
-    if constexpr (!BIAS) rs = sums(min(srow, 16u * MT - 1)) + 16 * (threadIdx.x & 3);
+    const uint8_t* const rs = sums(min(srow, 16u * MT - 1)) + 16 * (threadIdx.x & 3);
     uint8_t* const lds_sums = lds + (RESIDENT ? terms * chunks : 2) * (MT * 4096);
     const uint32_t to = row0 * 256 + 16 * (piece ^ row0);  // row0 + 16 i: 4096 bytes further each
-    u4v ra[MT], rw[AHEAD + 1][NT], rx{};
-    Q4Params<GPC> rp[AHEAD + 1][NT];
+    u4v ra[MT], rw[2][NT], rx{};
+    Q4Params<GPC> rp[2][NT];
     Q4Biases<SBF, GPC> biases[NT];
     struct Cursor {
         uint32_t cb, term, c;
@@ -202,7 +201,7 @@ __device__ __forceinline__ void q4_gemm(uint8_t* lds, const uint8_t* w, uint32_t
     for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) out[t][mt] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
-    Cursor at{cb, 0, 0}, far = at;  // the chunk that is multiplied, the one whose weights are read
+    Cursor at{cb, 0, 0};
     uint32_t buffer = 0;
     // one chunk; false after the last
     const auto step = [&](auto set_) __attribute__((always_inline)) {
@@ -215,7 +214,7 @@ __device__ __forceinline__ void q4_gemm(uint8_t* lds, const uint8_t* w, uint32_t
         // Eight groups' sums are read with the first of their chunks, and go to LDS a chunk later (a barrier after the other
         // buffer's last readers), or at once if no chunk follows: with one chunk in all, over the same values.
         uint8_t* const cycle_sums = lds_sums + (c / CYCLE & 1) * (MT * 1024);
-        if constexpr (!BIAS && !RESIDENT)
+        if constexpr (!RESIDENT)
             if (term == 0) {
                 if (c % CYCLE == 0) rx = *reinterpret_cast<const u4v*>(rs + c / CYCLE * 64);
                 if ((c % CYCLE == 1 || (c % CYCLE == 0 && c + 1 == chunks)) && srow < 16u * MT)
@@ -223,33 +222,29 @@ __device__ __forceinline__ void q4_gemm(uint8_t* lds, const uint8_t* w, uint32_t
             }
         if constexpr (!RESIDENT)
             if (more) load_rows(then.term, then.c);
-        if (inside(far)) {
-            load((SET + AHEAD) % (AHEAD + 1), far);
-            far = next(far);
-        }
+        if (more) load(1 - SET, then);
         if constexpr (!RESIDENT) __syncthreads();  // the chunk is staged; its buffer's last readers were before the last one
-        q4_gemm_chunk<BF, SBF, GPC, MT, NT, BIAS>(lds + (RESIDENT ? term * chunks + c : buffer) * (MT * 4096), rw[SET], rp[SET],
+        q4_gemm_chunk<BF, SBF, GPC, MT, NT, false>(lds + (RESIDENT ? term * chunks + c : buffer) * (MT * 4096), rw[SET], rp[SET],
                                                   lane, out);
-        if constexpr (!BIAS)
-            if (term == 0) {
+        if (term == 0) {
 #pragma unroll
-                for (int t = 0; t < NT; ++t) biases[t].take(rp[SET][t]);
-                if (c % CYCLE == CYCLE - 1 || c + 1 == chunks) {
-                    for (uint32_t i = c % CYCLE; i < CYCLE - 1; ++i) {  // no more chunks: zeros up to the eighth group
-                        constexpr Q4Params<GPC> none{};
+            for (int t = 0; t < NT; ++t) biases[t].take(rp[SET][t]);
+            if (c % CYCLE == CYCLE - 1 || c + 1 == chunks) {
+                for (uint32_t i = c % CYCLE; i < CYCLE - 1; ++i) {  // no more chunks: zeros up to the eighth group
+                    constexpr Q4Params<GPC> none{};
 #pragma unroll
-                        for (int t = 0; t < NT; ++t) biases[t].take(none);
-                    }
-                    u4v a[MT];
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) {
-                        const int r = mt * 16 + (lane & 15);
-                        a[mt] = *reinterpret_cast<const u4v*>(cycle_sums + 16 * (4 * r + ((lane >> 4) ^ (r >> 2 & 3))));
-                    }
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) biases[t].add(a, out[t]);
+                    for (int t = 0; t < NT; ++t) biases[t].take(none);
                 }
+                u4v a[MT];
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    const int r = mt * 16 + (lane & 15);
+                    a[mt] = *reinterpret_cast<const u4v*>(cycle_sums + 16 * (4 * r + ((lane >> 4) ^ (r >> 2 & 3))));
+                }
+#pragma unroll
+                for (int t = 0; t < NT; ++t) biases[t].add(a, out[t]);
             }
+        }
         if (ends) {
             const uint32_t tile0 = (at.cb * 4 + wave) * NT;
             if constexpr (TURN) {  // 16 rows of the wave's columns at a time, where the chunks were once no wave reads them
@@ -281,31 +276,20 @@ __device__ __forceinline__ void q4_gemm(uint8_t* lds, const uint8_t* w, uint32_t
         return more;
     };
     if constexpr (!RESIDENT) load_rows(0, 0);
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i)
-        if (inside(far)) {
-            load(i, far);
-            far = next(far);
-        }
+    load(0, at);
     if constexpr (RESIDENT) {
         for (uint32_t t = 0; t < terms; ++t)
             for (uint32_t ci = 0; ci < chunks; ++ci) {
                 load_rows(t, ci);
                 stage(t * chunks + ci);
             }
-        if constexpr (!BIAS)
-            for (uint32_t i = 0; i * CYCLE < chunks; ++i)
-                if (srow < 16u * MT)
-                    *reinterpret_cast<u4v*>(lds_sums + i * (MT * 1024) + sto) = *reinterpret_cast<const u4v*>(rs + i * 64);
+        for (uint32_t i = 0; i * CYCLE < chunks; ++i)
+            if (srow < 16u * MT)
+                *reinterpret_cast<u4v*>(lds_sums + i * (MT * 1024) + sto) = *reinterpret_cast<const u4v*>(rs + i * 64);
         __syncthreads();
     }
-    if constexpr (AHEAD == 1)
-        while (step(std::integral_constant<int, 0>{}) && step(std::integral_constant<int, 1>{})) {
-        }
-    else
-        while (step(std::integral_constant<int, 0>{}) && step(std::integral_constant<int, 1>{}) &&
-               step(std::integral_constant<int, 2>{})) {
-        }
+    while (step(std::integral_constant<int, 0>{}) && step(std::integral_constant<int, 1>{})) {
+    }
 }
 
 }  // namespace ea

@@ -314,6 +314,34 @@ def test_gpu_experts_sizes(ea, E, D, I, group, slots, R):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("E,D,I,group,slots,R,dt,out_dtype", [
+    (16, 256, 512, 64, 4, 1200, BF16, BF16), (16, 256, 512, 32, 4, 1200, F16, F32), (24, 128, 512, 128, 3, 1400, BF16, F32),
+    (8, 160, 1056, 32, 4, 900, BF16, F16), (4, 384, 2048, 128, 2, 1100, F16, F16), (40, 96, 320, 32, 8, 1000, F16, BF16),
+    (24, 1152, 384, 64, 3, 1700, BF16, BF16), (16, 128, 256, 64, 4, 2300, BF16, F16), (16, 192, 256, 32, 4, 2300, F16, F32),
+    (12, 64, 128, 32, 8, 2100, BF16, BF16), (16, 256, 512, 64, 4, 500, BF16, BF16)])
+def test_gpu_experts_long_items(ea, E, D, I, group, slots, R, dt, out_dtype):
+    """Prompts: items of up to 64 pairs of experts picked more and less often (some by nobody, some rows empty), widths whose
+    rows stay in LDS and wider ones; the same bits again, and for the rows in another order."""
+    g = torch.Generator().manual_seed(E + R)
+    mats = _layer(g, E, D, I, group, dt)
+    x = torch.randn((R, D), generator=g).to(dt)
+    heat = torch.rand((R, E), generator=g).log() / torch.linspace(3.0, 0.05, E)
+    heat[:, 1] = float("-inf")
+    pick = heat.topk(slots, dim=1).indices.to(torch.int32)
+    wts = torch.rand((R, slots), generator=g) + 0.1
+    pick[R - 20:] = -1
+    out, ex, sc = _experts(ea, x, pick, wts, mats, out_dtype, pad=8)
+    want, err = plain.experts(x.double(), pick, wts, *mats, out_dtype)
+    plain.close(out, want, err)
+    assert (out[R - 20:] == 0).all()
+    again, _, _ = _experts(ea, x, pick, wts, mats, out_dtype, ex=ex, sc=sc)
+    assert torch.equal(out, again)
+    order = torch.randperm(R, generator=g)
+    turned, _, _ = _experts(ea, x[order], pick[order], wts[order], mats, out_dtype, ex=ex, sc=sc)
+    assert torch.equal(out[order.cuda()], turned)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("R", [1, 6, 16, 17, 150])
 def test_gpu_experts_odd_picks(ea, R):
     """Empty slots and rows, picks outside the experts, one expert for all, an expert twice in a row; NaN weights and rows
