@@ -241,7 +241,7 @@ int ea_q4_call(ea_stream_t stream, const ea_q4_linear* const* ls, uint32_t nls, 
     uint32_t tiles = 0;
     for (uint32_t j = 0; j < nls; ++j) {
         const ea_q4_linear* l = ls[j];
-        if (!l || !l->words || !outs[j] || out_dtypes[j] < F16 || out_dtypes[j] > F32) return EA_BAD_ARGUMENT;
+        if (!l || !l->words || (l->words & 15) || !outs[j] || out_dtypes[j] < F16 || out_dtypes[j] > F32) return EA_BAD_ARGUMENT;
         if (!q4_group_ok(l->group)) return EA_BAD_WIDTH;
         if (l->n == 0 || l->k == 0 || (l->s_dtype != F16 && l->s_dtype != BF16)) return EA_BAD_ARGUMENT;
         if (l->k % l->group != 0) return EA_UNEVEN_SPLIT;

@@ -581,7 +581,7 @@ static uint32_t q4_max_items(uint32_t experts, size_t pairs, uint32_t item = Q4_
 }
 
 static int q4_experts_ok(const ea_q4_experts* ex) {
-    if (!ex || !ex->gu || !ex->down || (ex->s_dtype != F16 && ex->s_dtype != BF16)) return EA_BAD_ARGUMENT;
+    if (!ex || !ex->gu || !ex->down || ((ex->gu | ex->down) & 15) || (ex->s_dtype != F16 && ex->s_dtype != BF16)) return EA_BAD_ARGUMENT;
     if (ex->group != 32 && ex->group != 64 && ex->group != 128) return EA_BAD_WIDTH;
     if (ex->count == 0 || ex->dims == 0 || ex->width == 0) return EA_BAD_ARGUMENT;
     if (ex->count > Q4_MAX_EXPERTS) return EA_TOO_MANY_EXPERTS;

@@ -293,8 +293,8 @@ enum { EA_SCORE_SIGMOID = 0, EA_SCORE_SOFTMAX = 1 };
  * (the lower run among runs); wts = score of the pick, divided by (their sum + 1e-20) with renorm, times scale. Scores and
  * choices are held in 64 bits, so the picks do not depend on how a 32-bit score rounds; wts is rounded once.
  * An expert whose logit is -inf is out: it is never picked, it gives its run nothing, and where fewer than `slots` are left
- * the slots behind get pick -1 and weight 0 (a slot without an expert for ea_q4_routed and ea_moe_routed). A NaN choice ranks
- * below every number, NaNs by the lower expert. 1..EA_ROUTE_MAX_EXPERTS experts, 1..32 slots (EA_TOO_MANY_SLOTS: more, or
+ * the slots behind get pick -1 and weight 0: a slot without an expert for ea_q4_routed (the EXL3 experts' calls take experts
+ * only). A NaN choice ranks below every number, NaNs by the lower expert. 1..EA_ROUTE_MAX_EXPERTS experts, 1..32 slots (EA_TOO_MANY_SLOTS: more, or
  * more than the kept runs hold), 1..64 groups that divide experts (EA_UNEVEN_SPLIT). No counterpart in the reference, whose
  * router is ea_topk8's alone. */
 int ea_route(ea_stream_t stream, const void* logits, int l_dtype, uint32_t l_stride, const float* bias, int32_t* pick,
@@ -323,7 +323,7 @@ int ea_q4_pack(ea_stream_t stream, const void* words0, const void* scales0, cons
                uint32_t count);
 
 typedef struct ea_q4_linear {
-    uint64_t words;               /* ea_q4_pack's output */
+    uint64_t words;               /* ea_q4_pack's output, 16-byte aligned */
     uint32_t k, n, group;
     int32_t s_dtype;
 } ea_q4_linear;
@@ -333,7 +333,7 @@ typedef struct ea_q4_linear {
 int ea_q4_call(ea_stream_t stream, const ea_q4_linear* const* ls, uint32_t nls, const void* x, int x_dtype,
                uint32_t x_stride, uint32_t m, const uint64_t* outs, const int* out_dtypes);
 
-/* One layer's routed experts: gate | up packed together ([count] x ea_q4_bytes(16 * ceil(width / 8), dims, group)) and down
+/* One layer's routed experts, 16-byte aligned: gate | up packed together ([count] x ea_q4_bytes(16 * ceil(width / 8), dims, group)) and down
  * ([count] x ea_q4_bytes(dims, width, group)). dims and width are multiples of group; at most 4096 experts. */
 typedef struct ea_q4_experts {
     uint64_t gu, down;

@@ -57,7 +57,7 @@ def test_call_refuses():
     assert _call([_lin()], x_stride=124) == 9 and _call([_lin()], x_stride=130) == 9
     for bad in (dict(x=0), dict(x=4098), dict(x=4100), dict(x_dtype=2), dict(outs=[0]), dict(dts=[3]), dict(m=65537)):
         assert _call([_lin()], **bad) == 18, bad
-    for bad in (dict(words=0), dict(n=0), dict(k=0), dict(s_dtype=2)):
+    for bad in (dict(words=0), dict(words=4104), dict(n=0), dict(k=0), dict(s_dtype=2)):
         assert _call([_lin(**bad)]) == 18, bad
     if not torch.cuda.is_available():
         assert _call([_lin()]) == 17
@@ -83,9 +83,9 @@ def test_experts_refuse():
     assert init(size=n - 1) == 12 and init(base=0) == 18 and init(base=4097) == 18 and init(slots=33) == 6
     assert init(slots=0) == 6 and init(rows=0) == 18 and init(rows=262145, size=1 << 60) == 18
     for e, code in ((_ex(group=48), 11), (_ex(dims=224), 8), (_ex(width=96), 8), (_ex(count=0), 18), (_ex(count=4097), 5),
-                    (_ex(gu=0), 18), (_ex(down=0), 18), (_ex(s_dtype=2), 18), (_ex(dims=0), 18)):
+                    (_ex(gu=0), 18), (_ex(down=0), 18), (_ex(gu=4104), 18), (_ex(down=4100), 18), (_ex(s_dtype=2), 18), (_ex(dims=0), 18)):
         assert init(e) == code
-        assert L.ea_q4_scratch_bytes(C.byref(e), 8, 2) == 0 or e.gu == 0 or e.down == 0
+        assert L.ea_q4_scratch_bytes(C.byref(e), 8, 2) == 0
     assert init() == 0
 
     def call(e=ex, x=4096, x_dtype=1, stride=256, pick=4096, wts=4096, s=sc, out=4096, dt=2, R=1):
@@ -407,6 +407,54 @@ def test_gpu_experts_same_bits_again(ea, R):
         order = torch.randperm(R, generator=g)
         b, _, _ = _experts(ea, x[order], pick[order], wts[order], mats, F32, ex=ex, sc=sc)
         assert torch.equal(a[order.cuda()], b)
+
+
+@pytest.mark.gpu
+def test_gpu_experts_on_two_streams(ea):
+    """Two layers at once, each with a stream and a scratch of its own, from one row to long items; and a captured prompt pass
+    replayed between eager ones on the same scratch."""
+    device, ops, q4 = ea
+    g = torch.Generator().manual_seed(3)
+    E, D, I, S = 16, 256, 512, 4
+    exs = [q4.Experts(*(_cuda(m) for m in _layer(g, E, D, I, 64, BF16))) for _ in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for R in (1, 16, 100, 1200):
+        scs = [q4.Scratch(ex, R, S) for ex in exs]
+        xs = [torch.randn((R, D), generator=g).to(BF16).cuda() for _ in exs]
+        routing = [[t.cuda() for t in _routing(g, R, E, S)] for _ in exs]
+        outs = [torch.zeros((R, D), device="cuda") for _ in exs]
+
+        def run(i, stream):
+            q4.routed(stream, xs[i].data_ptr(), 1, D, routing[i][0].data_ptr(), routing[i][1].data_ptr(), exs[i], scs[i],
+                      outs[i].data_ptr(), 2, R)
+
+        torch.cuda.synchronize()
+        want = []
+        for i in range(2):
+            run(i, device.stream())
+            want.append(outs[i].clone())
+        torch.cuda.synchronize()
+        for o in outs:
+            o.fill_(5)
+        torch.cuda.synchronize()
+        for _ in range(4):
+            for i in range(2):
+                run(i, device.stream(streams[i]))
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=streams[0]):
+            run(0, device.stream())
+        for _ in range(3):
+            outs[0].fill_(5)
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(outs[0], want[0])
+            xs[0].neg_()
+            run(0, device.stream())
+            xs[0].neg_()
+            torch.cuda.synchronize()
 
 
 # ---- the set together -----------------------------------------------------------------------------------------------
