@@ -73,11 +73,13 @@ struct Q4LinArgs {
     int jobs;
 };
 
-// Up to 16 rows: a block takes NT tiles of one job and all rows; its WK waves take every WK-th chunk and add their sums in wave
+// Few rows: a block takes NT tiles of one job and up to 16 rows; its WK waves take every WK-th chunk and add their sums in wave
 // order. Bound by the weights' bandwidth where there are many, by latencies where there are few; from then on by the rows,
 // which every block reads from L2, so wide jobs take four tiles a block, which share them: 65521 x 6144 at 1 / 8 / 16 rows
-// 41 / 46 / 54 us with four tiles (226 MB: 5.5 TB/s), 44 / 55 / 74 with two, 57 / 86 / 118 with one; but 8192 x 6144 at one row
-// 12.3, 9.9 and 9.4 us, where four tiles leave half of the card idle. 2048 x 6144: 5.4 us with 16 waves a tile.
+// 41 / 46 / 54 us with four tiles (226 MB: 5.5 TB/s), 44 / 55 / 74 with two, 57 / 86 / 118 with one; 8192 x 6144 at one row
+// 11.3, 8.4 and 9.6 us, 4096 x 6144 9.8, 6.7 and 5.6, where more tiles a block leave the card idle. 2048 x 6144: 5.4 us.
+// More than 16 rows are cut into groups of 16 where all blocks then run at once and a row is long: 32 rows x 2048 x 6144 take
+// 9.0 us so, 14.4 in blocks of 32 rows; but 48 rows 15.0 and 14.6, and 64 x 512 x 2048 8.1 and 7.3.
 template <bool BF, bool SBF, int GPC, int NT, int WK, int NB>
 __global__ void __launch_bounds__(64 * WK) q4_linear_kernel(Q4LinArgs a) {
     __shared__ f4v part[WK][NT][64];
@@ -87,7 +89,8 @@ __global__ void __launch_bounds__(64 * WK) q4_linear_kernel(Q4LinArgs a) {
     if (tile0 >= tiles) return;
     const size_t tile_bytes = (size_t)a.chunks * q4_chunk_bytes(GPC);
     const uint32_t first = min(tile0, tiles - min(tiles, (uint32_t)NT));  // the last block's tiles overlap
-    const uint16_t* row = a.x + (size_t)min((uint32_t)(lane & 15), a.m - 1) * a.x_stride;  // rows past m re-read the last
+    const uint32_t m0 = blockIdx.y * 16, m = min(a.m - m0, 16u);
+    const uint16_t* row = a.x + (size_t)(m0 + min((uint32_t)(lane & 15), m - 1)) * a.x_stride;  // past m the last row again
     f4v out[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) out[t] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
@@ -96,17 +99,20 @@ __global__ void __launch_bounds__(64 * WK) q4_linear_kernel(Q4LinArgs a) {
 #pragma unroll
     for (int t = 0; t < NT; ++t) part[wave][t][lane] = out[t];
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < 16 * NT * a.m; i += 64 * WK) {
+    for (uint32_t i = threadIdx.x; i < 16 * NT * m; i += 64 * WK) {
         const uint32_t n = i & 15, t = (i >> 4) % NT, r = i / (16 * NT), col = (first + t) * 16 + n;
-        if (col < job.n) store_act(job.y, job.y_dtype, (size_t)r * job.n + col, q4_total<WK, NT>(part, t, r, n));
+        if (col < job.n) store_act(job.y, job.y_dtype, (size_t)(m0 + r) * job.n + col, q4_total<WK, NT>(part, t, r, n));
     }
 }
 
 // More rows: a block takes 16 MT rows and 4 NT tiles, and KS groups of four waves every KS-th chunk of them: each group stages
 // its chunk's rows in LDS, in two buffers, while the chunk before is multiplied, and reads its weights a chunk ahead; the
-// groups' sums are added in order at the end. Matrix and vector instructions hardly overlap here (measured: a product takes 17
-// cycles, a vector instruction 2.4 to 4.5, and together their sum), so waves count more than large tiles: 512 rows x 12000 x
-// 8192 take 189 us with 32 rows, two tiles and two groups, 198 with 64 rows, 212 without groups.
+// groups' sums are added in order at the end. Four groups of one tile a wave where that makes at most 256 blocks, else two of
+// two tiles: 128 rows x 2048 x 6144 15.4 against 24.8 us, 64 x 8192 x 2048 8.7 against 11.8, but 128 x 6144 x 2048 13.7
+// against 12.5, 301 x 6144 x 2048 26.5 against 19 (400 TFLOP/s). Matrix and vector instructions hardly overlap here
+// (measured: a product takes 17 cycles, a vector instruction 2.4 to 4.5, and together their sum), so waves count more than
+// large tiles: 512 rows x 12000 x 8192 take 189 us with 32 rows, two tiles and two groups, 198 with 64 rows, 212 without
+// groups.
 template <bool BF, bool SBF, int GPC, int MT, int NT, int KS>
 __global__ void __launch_bounds__(256 * KS) q4_linear_split_kernel(Q4LinArgs a) {
     constexpr int BUFFER = MT * 4096, PARTS = KS * 4 * NT * MT * 1024;
@@ -181,16 +187,19 @@ static int launch_linear(hipStream_t s, const Q4LinArgs& a, uint32_t tiles, bool
         constexpr int GPC = decltype(gpc_)::value;
         constexpr bool BF = decltype(bf_)::value, SBF = decltype(sbf_)::value;
         const unsigned jobs = (unsigned)a.jobs;
-        const auto blocks = [&](uint32_t rows, uint32_t nt) { return dim3((tiles + 4 * nt - 1) / (4 * nt), (a.m + rows - 1) / rows, jobs); };
-        if (a.m <= 16) {
-            if (tiles * jobs < 512) q4_linear_kernel<BF, SBF, GPC, 1, 16, 3><<<dim3(tiles, 1, jobs), 1024, 0, s>>>(a);
-            else if (tiles * jobs < 1536) q4_linear_kernel<BF, SBF, GPC, 2, 8, 3><<<dim3((tiles + 1) / 2, 1, jobs), 512, 0, s>>>(a);
-            else q4_linear_kernel<BF, SBF, GPC, 4, 8, 2><<<dim3((tiles + 3) / 4, 1, jobs), 512, 0, s>>>(a);
+        const unsigned groups = (a.m + 15) / 16;
+        const auto blocks = [&](uint32_t nt, uint32_t rows) {
+            return dim3((tiles + nt - 1) / nt, (a.m + rows - 1) / rows, jobs);
+        };
+        if (groups == 1 || ((uint64_t)tiles * jobs * groups <= 256 && a.chunks > 16)) {
+            if (tiles * jobs < 512) q4_linear_kernel<BF, SBF, GPC, 1, 16, 3><<<blocks(1, 16), 1024, 0, s>>>(a);
+            else if (tiles * jobs < 1536) q4_linear_kernel<BF, SBF, GPC, 2, 8, 3><<<blocks(2, 16), 512, 0, s>>>(a);
+            else q4_linear_kernel<BF, SBF, GPC, 4, 8, 2><<<blocks(4, 16), 512, 0, s>>>(a);
             return;
         }
-        const dim3 one = blocks(32, 1);
-        if (one.x * one.y * jobs <= 256) q4_linear_split_kernel<BF, SBF, GPC, 2, 1, 4><<<one, 1024, 0, s>>>(a);
-        else q4_linear_split_kernel<BF, SBF, GPC, 2, 2, 2><<<blocks(32, 2), 512, 0, s>>>(a);
+        const dim3 one = blocks(4, 32);  // four waves of a tile each
+        if ((uint64_t)one.x * one.y * jobs <= 256) q4_linear_split_kernel<BF, SBF, GPC, 2, 1, 4><<<one, 1024, 0, s>>>(a);
+        else q4_linear_split_kernel<BF, SBF, GPC, 2, 2, 2><<<blocks(8, 32), 512, 0, s>>>(a);
     };
     q4_types(bf, sbf, gpc, go);
     return launched();
@@ -241,7 +250,8 @@ int ea_q4_call(ea_stream_t stream, const ea_q4_linear* const* ls, uint32_t nls, 
     uint32_t tiles = 0;
     for (uint32_t j = 0; j < nls; ++j) {
         const ea_q4_linear* l = ls[j];
-        if (!l || !l->words || (l->words & 15) || !outs[j] || out_dtypes[j] < F16 || out_dtypes[j] > F32) return EA_BAD_ARGUMENT;
+        if (!l || !l->words || (l->words & 15) || !outs[j]) return EA_BAD_ARGUMENT;
+        if (out_dtypes[j] < F16 || out_dtypes[j] > F32) return EA_BAD_ARGUMENT;
         if (!q4_group_ok(l->group)) return EA_BAD_WIDTH;
         if (l->n == 0 || l->k == 0 || (l->s_dtype != F16 && l->s_dtype != BF16)) return EA_BAD_ARGUMENT;
         if (l->k % l->group != 0) return EA_UNEVEN_SPLIT;

@@ -3,7 +3,12 @@
 // The rows' picks are sorted by expert and cut into items (an expert and up to 16 of its pairs); a block multiplies an
 // item's rows by tiles of the expert's gate|up (8 columns of each) and writes the activated pairs; another multiplies those
 // by tiles of the down projection; the last launch adds a row's slots in order. A pair's values depend neither on the others
-// of its item nor on their order, so the results are the same on every run.
+// of its item nor on their order, so the results are the same on every run. Where experts have many rows, items are of up
+// to 64 pairs (long items), which turn a weight into a matrix operand once for all of them.
+//
+// A pair takes 6 D I operations, an expert that is picked 3 D I / 2 bytes of words and 12 D I / group of scales and biases: up
+// to some tens of rows the weights' bytes bound it, at one row latencies. Figures in this file: D 6144, I 256, 256 experts,
+// 8 picks a row, groups of 64, bf16 in and out: 1.77 MB gate|up and 0.88 MB down an expert.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -46,7 +51,8 @@ struct Q4MoeArgs {
 // ---- grouping -----------------------------------------------------------------------------------------------------
 // One block: the pairs of each expert counted, the items before each expert scanned, the pairs placed (in any order within an
 // expert). Full items come before all others, so that the longest work starts first. A pick outside 0 .. experts - 1 is a slot
-// without an expert.
+// without an expert. Bound by its passes' latencies: 5 us at 64 rows, 12 at 512, 15 at 2048 (with items in four classes of
+// size instead of two 24, and 3 % less in the products behind).
 __device__ void q4_group(const Q4MoeArgs& a) {
     __shared__ uint32_t count[Q4_MAX_EXPERTS], full[Q4_MAX_EXPERTS], rest[Q4_MAX_EXPERTS], sums[2][16], all;
     __shared__ uint16_t nfull[Q4_MAX_EXPERTS];  // at most EA_Q4_MAX_PAIRS / Q4_ITEM
@@ -203,7 +209,10 @@ __device__ __forceinline__ void store_terms(uint16_t* h, int terms, size_t plane
 // Block (NT tiles of gate | up, item): 16 rows of a matrix instruction, those that the item does not have as zeros, which
 // cost neither loads nor cache; WK waves take every WK-th chunk. Up to 16 rows nothing is sorted before: block (tiles, pair)
 // works if no earlier pair names its expert, a row of the instruction is the row of x, and one more block groups the pairs
-// for the launches behind.
+// for the launches behind. One row: 6.0 us (2.4 TB/s; the launch, the pick, the weights, the sums after each other). 16 rows
+// 43 us (102 experts, 4.2 TB/s), 64 rows, in items, 77 us (5.1 TB/s, above what a large copy reaches). From two rows on two
+// tiles a block share their reads of x: 2 / 4 / 8 / 16 rows 9.7 / 14.1 / 25.8 / 42.7 us, with one tile 10.4 / 16.6 / 31.7 /
+// 55.6.
 enum Q4Rows { ONE_ROW, FEW_ROWS, ITEMS };
 
 template <bool BF, bool SBF, int GPC, int NT, int WK, int NB, int MODE>
@@ -277,7 +286,8 @@ __global__ void __launch_bounds__(64 * WK) q4_gateup_kernel(Q4MoeArgs a) {
 
 // ---- down -----------------------------------------------------------------------------------------------------------
 // One row: NT tiles of the output a block; its waves take the (slot, chunk) units in turn, weigh their sums in registers, and
-// terms (rows 0 .. TERMS - 1 of the instruction) and waves are added at the end.
+// terms (rows 0 .. TERMS - 1 of the instruction) and waves are added at the end: nothing is left for a launch behind.
+// 4.6 us (1.5 TB/s): the launch, picks, weights and sums after each other.
 template <bool SBF, int GPC, int TERMS, int NT, int WK, int NB>
 __global__ void __launch_bounds__(64 * WK) q4_down_one_kernel(Q4MoeArgs a) {
     __shared__ f4v part[WK][NT][64];
@@ -353,7 +363,7 @@ __global__ void __launch_bounds__(64 * WK) q4_down_one_kernel(Q4MoeArgs a) {
 // expert's weights are read where they lie together (blocks that took some tiles of every expert read them at half the rate).
 // Terms are rows of their own: rows 4 q .. 4 q + 3 of the instruction are quad q of the accumulators' lanes; with three
 // terms quad q holds term q of four pairs, with two quads 2 q and 2 q + 1 term q of eight, and adding lanes 16 (and 32)
-// apart adds the terms.
+// apart adds the terms. 16 rows 21 us (4.3 TB/s), 64 rows 44 us (4.5 TB/s): the weights, and a pair's fp32 sums, 24 KB each.
 template <bool SBF, int GPC, int TERMS, int NT, int WK, int NB>
 __global__ void __launch_bounds__(64 * WK) q4_down_kernel(Q4MoeArgs a) {
     constexpr int PER = TERMS == 1 ? 16 : TERMS == 2 ? 8 : 4;  // pairs a product
@@ -412,15 +422,21 @@ template <bool BF, bool SBF, int GPC, int NT4, int NT, bool RESIDENT, bool TURN,
 __device__ __forceinline__ void q4_item_gemm(uint8_t* lds, int count, const uint8_t* w, uint32_t tiles, uint32_t k,
                                              uint32_t terms, size_t plane, uint32_t cb, uint32_t cb_step, ROW row,
                                              SUMS sums, STORE store) {
-    if (count > 32) q4_gemm<BF, SBF, GPC, 4, NT4, RESIDENT, TURN>(lds, w, tiles, k, terms, plane, cb, cb_step, row, sums, store);
+    const auto go = [&](auto mt_, auto nt_) __attribute__((always_inline)) {
+        q4_gemm<BF, SBF, GPC, decltype(mt_)::value, decltype(nt_)::value, RESIDENT, TURN>(lds, w, tiles, k, terms, plane, cb,
+                                                                                        cb_step, row, sums, store);
+    };
+    if (count > 32) go(std::integral_constant<int, 4>{}, std::integral_constant<int, NT4>{});
     else if (cb * 4 * NT >= tiles) return;
-    else if (count > 16) q4_gemm<BF, SBF, GPC, 2, NT, RESIDENT, TURN>(lds, w, tiles, k, terms, plane, cb, cb_step, row, sums, store);
-    else q4_gemm<BF, SBF, GPC, 1, NT, RESIDENT, TURN>(lds, w, tiles, k, terms, plane, cb, cb_step, row, sums, store);
+    else if (count > 16) go(std::integral_constant<int, 2>{}, std::integral_constant<int, NT>{});
+    else go(std::integral_constant<int, 1>{}, std::integral_constant<int, NT>{});
 }
 
 // Blocks go to the card's eight dies in turn, and each die has an L2 of its own: die x takes the x-th eighth of the full items
-// (of the partial ones), a run by expert, and all column blocks of its items, so that an expert's weights and an item's rows
-// come from memory once a die.
+// (of the partial ones), a run by expert, and all column blocks of its items, so that an expert's items share its weights on
+// one die. Column blocks are the slow index: blocks behind an item's last one return at once, and where those come at a
+// fixed distance they fall on the same shader engines, which leaves half of the card idle (gate|up, 256 rows: 167 against
+// 96 us).
 struct Q4Place {
     int item;  // -1: none
     uint32_t cb;
@@ -439,6 +455,10 @@ __device__ __forceinline__ Q4Place q4_place(const Q4MoeArgs& a, uint32_t blocks)
 }
 static unsigned q4_place_blocks(uint32_t max_items, uint32_t blocks) { return Q4_DIES * (max_items / Q4_DIES + 2) * blocks; }
 
+// Two tiles a wave with more than 32 rows, else four: 2048 rows 265 us (390 TFLOP/s), with four throughout 290. Matrix
+// instructions alone would take a third of that; conversions and scalings hardly overlap them, every operand comes from LDS
+// for two products only, and blocks end unevenly: items of up to 80 or 96 rows, which convert fewer weights, take as long
+// (266, 280) at 2048 rows and longer (206, 218 against 185) at 1024.
 template <bool BF, bool SBF, int GPC, int NT4, int NT>
 __global__ void __launch_bounds__(Q4_GEMM_THREADS, 2) q4_gateup_gemm_kernel(Q4MoeArgs a, uint32_t blocks) {
     __shared__ __attribute__((aligned(16))) uint8_t lds[std::max(q4_gemm_lds<4, NT4>(), q4_gemm_lds<2, NT>())];
@@ -446,10 +466,11 @@ __global__ void __launch_bounds__(Q4_GEMM_THREADS, 2) q4_gateup_gemm_kernel(Q4Mo
     if (at.item < 0) return;
     const Q4Item& it = a.items[at.item];
     const int e = it.expert, count = it.count;
+    const auto row_of = [&](int i) { return (size_t)((uint32_t)it.pair[min(i, count - 1)] / a.slots); };
     q4_item_gemm<BF, SBF, GPC, NT4, NT, false, false>(
         lds, count, a.gu + (size_t)e * a.gu_bytes, (a.width + 7) / 8, a.dims, 1, 0, at.cb, 1u << 24,
-        [&](int i) { return a.x + (size_t)((uint32_t)it.pair[min(i, count - 1)] / a.slots) * a.x_stride; },
-        [&](int i) { return a.xsums + (size_t)((uint32_t)it.pair[min(i, count - 1)] / a.slots) * q4_sum_bytes(a.dims / a.group); },
+        [&](int i) { return a.x + row_of(i) * a.x_stride; },
+        [&](int i) { return a.xsums + row_of(i) * q4_sum_bytes(a.dims / a.group); },
         [&](uint32_t tile, const auto& v) {
             const int lane = threadIdx.x & 63;
             const uint32_t col = tile * 8 + (lane & 7);
@@ -466,6 +487,10 @@ __global__ void __launch_bounds__(Q4_GEMM_THREADS, 2) q4_gateup_gemm_kernel(Q4Mo
         });
 }
 
+// A block takes every `blocks`-th column block of an item, six blocks an item at most, and with RESIDENT keeps its rows in LDS
+// meanwhile. 2048 rows 175 us: 403 MB of fp32 sums written and 226 MB of weights read (3.6 TB/s). In two launches of half the
+// columns, each with its sums over slots behind, which then find them in the last-level cache, both together take 266
+// instead of 274 us at 2048 rows, but 183 instead of 157 at 1024.
 template <bool SBF, int GPC, int NT, bool RESIDENT>
 __global__ void __launch_bounds__(Q4_GEMM_THREADS, 2) q4_down_gemm_kernel(Q4MoeArgs a, uint32_t blocks) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
@@ -483,6 +508,7 @@ __global__ void __launch_bounds__(Q4_GEMM_THREADS, 2) q4_down_gemm_kernel(Q4MoeA
 }
 
 // ---- a row's slots, in order ----------------------------------------------------------------------------------------
+// Bound by the pairs' sums: 64 rows 5 us (12.6 MB), 2048 rows 85 to 98 us (403 MB read, 25 MB written: 5.0 to 4.4 TB/s).
 __global__ void __launch_bounds__(256) q4_combine_kernel(Q4MoeArgs a) {
     __shared__ int32_t pick[32];
     __shared__ float weight[32];
@@ -539,12 +565,15 @@ static void launch_gateup(hipStream_t s, const Q4MoeArgs& a, bool bf, bool sbf, 
         constexpr bool BF = decltype(bf_)::value, SBF = decltype(sbf_)::value;
         constexpr int GPC = decltype(gpc_)::value;
         const dim3 one(tiles, a.pairs + (a.rows > 1)), two((tiles + 1) / 2, a.pairs + 1);
+        const bool few = a.rows <= Q4_ROWS;
         if (a.rows == 1) q4_gateup_kernel<BF, SBF, GPC, 1, 8, 3, ONE_ROW><<<one, 512, 0, s>>>(a);
-        else if (a.rows <= 4 || (a.rows <= Q4_ROWS && tiles < 2)) q4_gateup_kernel<BF, SBF, GPC, 1, 8, 3, FEW_ROWS><<<one, 512, 0, s>>>(a);
-        else if (a.rows <= Q4_ROWS) q4_gateup_kernel<BF, SBF, GPC, 2, 8, 3, FEW_ROWS><<<two, 512, 0, s>>>(a);
-        else if (a.item == Q4_BIG_ITEM)
-            q4_gateup_gemm_kernel<BF, SBF, GPC, 2, 4><<<q4_place_blocks(max_items, (tiles + 7) / 8), Q4_GEMM_THREADS, 0, s>>>(a, (tiles + 7) / 8);
-        else if (tiles < 2) q4_gateup_kernel<BF, SBF, GPC, 1, 8, 3, ITEMS><<<dim3(1, max_items), 512, 0, s>>>(a);
+        else if (few && tiles < 2) q4_gateup_kernel<BF, SBF, GPC, 1, 8, 3, FEW_ROWS><<<one, 512, 0, s>>>(a);
+        else if (few) q4_gateup_kernel<BF, SBF, GPC, 2, 8, 3, FEW_ROWS><<<two, 512, 0, s>>>(a);
+        else if (a.item == Q4_BIG_ITEM) {
+            const uint32_t blocks = (tiles + 7) / 8;
+            const unsigned grid = q4_place_blocks(max_items, blocks);
+            q4_gateup_gemm_kernel<BF, SBF, GPC, 2, 4><<<grid, Q4_GEMM_THREADS, 0, s>>>(a, blocks);
+        } else if (tiles < 2) q4_gateup_kernel<BF, SBF, GPC, 1, 8, 3, ITEMS><<<dim3(1, max_items), 512, 0, s>>>(a);
         else q4_gateup_kernel<BF, SBF, GPC, 2, 8, 3, ITEMS><<<dim3((tiles + 1) / 2, max_items), 512, 0, s>>>(a);
     });
 }
@@ -557,22 +586,22 @@ static void launch_down(hipStream_t s, const Q4MoeArgs& a, bool sbf, int gpc, ui
             constexpr bool SBF = decltype(sbf_)::value;
             constexpr int GPC = decltype(gpc_)::value;
             if (a.rows == 1) q4_down_one_kernel<SBF, GPC, TERMS, 1, 8, 2><<<tiles, 512, 0, s>>>(a);
-            else if (a.item == Q4_BIG_ITEM)
-                [&] {
-                    const uint32_t blocks = std::min((tiles + 15) / 16, 6u);
-                    const unsigned grid = q4_place_blocks(max_items, blocks);
-                    const uint32_t buffers = TERMS * q4_chunks(a.width);
-                    if (buffers <= Q4_RESIDENT)
-                        q4_down_gemm_kernel<SBF, GPC, 4, true><<<grid, Q4_GEMM_THREADS, q4_gemm_lds<4, 4>(buffers), s>>>(a, blocks);
-                    else q4_down_gemm_kernel<SBF, GPC, 4, false><<<grid, Q4_GEMM_THREADS, q4_gemm_lds<4, 4>(), s>>>(a, blocks);
-                }();
-            else if (tiles >= 4) q4_down_kernel<SBF, GPC, TERMS, 4, 8, 1><<<dim3((tiles + 31) / 32, max_items), 512, 0, s>>>(a);
+            else if (a.item == Q4_BIG_ITEM) {
+                const uint32_t blocks = std::min((tiles + 15) / 16, 6u), buffers = TERMS * q4_chunks(a.width);
+                const unsigned grid = q4_place_blocks(max_items, blocks);
+                if (buffers <= Q4_RESIDENT)
+                    q4_down_gemm_kernel<SBF, GPC, 4, true>
+                        <<<grid, Q4_GEMM_THREADS, q4_gemm_lds<4, 4>((int)buffers), s>>>(a, blocks);
+                else q4_down_gemm_kernel<SBF, GPC, 4, false><<<grid, Q4_GEMM_THREADS, q4_gemm_lds<4, 4>(), s>>>(a, blocks);
+            } else if (tiles >= 4) q4_down_kernel<SBF, GPC, TERMS, 4, 8, 1><<<dim3((tiles + 31) / 32, max_items), 512, 0, s>>>(a);
             else q4_down_kernel<SBF, GPC, TERMS, 1, 4, 1><<<dim3((tiles + 3) / 4, max_items), 256, 0, s>>>(a);
         }
     });
 }
 
-// Terms of the activated values: what the output's type can show (bf16 8 bits, fp16 11, fp32 24).
+// Terms of the activated values: what the output's type can show (bf16 8 bits, fp16 11, fp32 24). So with bf16 out h is
+// rounded once, as a layer in bf16 does; a second term would take 2 to 5 % at few rows and, at 2048, the down products from
+// 177 to 368 us.
 static int q4_terms(int out_dtype) { return out_dtype == BF16 ? 1 : out_dtype == F16 ? 2 : 3; }
 
 static uint32_t q4_max_items(uint32_t experts, size_t pairs, uint32_t item = Q4_ITEM) {
@@ -581,7 +610,8 @@ static uint32_t q4_max_items(uint32_t experts, size_t pairs, uint32_t item = Q4_
 }
 
 static int q4_experts_ok(const ea_q4_experts* ex) {
-    if (!ex || !ex->gu || !ex->down || ((ex->gu | ex->down) & 15) || (ex->s_dtype != F16 && ex->s_dtype != BF16)) return EA_BAD_ARGUMENT;
+    if (!ex || !ex->gu || !ex->down || ((ex->gu | ex->down) & 15)) return EA_BAD_ARGUMENT;
+    if (ex->s_dtype != F16 && ex->s_dtype != BF16) return EA_BAD_ARGUMENT;
     if (ex->group != 32 && ex->group != 64 && ex->group != 128) return EA_BAD_WIDTH;
     if (ex->count == 0 || ex->dims == 0 || ex->width == 0) return EA_BAD_ARGUMENT;
     if (ex->count > Q4_MAX_EXPERTS) return EA_TOO_MANY_EXPERTS;
@@ -677,7 +707,9 @@ int ea_q4_routed(ea_stream_t stream, const void* x, int x_dtype, uint32_t x_stri
     a.slots = sc->slots;
     a.out_dtype = out_dtype;
     a.terms = q4_terms(out_dtype);
-        // Long items pay where experts have several rows each and there are blocks enough for a row of chunks apiece.
+    // Long items pay where experts have more than about ten rows each, so that items of 16 would turn most weights twice, and
+    // where there are blocks enough to fill the card, as an item's waves no longer share a tile's chunks. All launches with
+    // short / long items: 256 rows 190 / 195 us, 320 201 / 196, 384 220 / 210, 512 279 / 220, 2048 847 / 563.
     const uint64_t some = std::min<uint64_t>(a.pairs, a.experts), column_blocks = ((a.width + 7) / 8 + 7) / 8;
     const bool big = R > Q4_ROWS && a.pairs > 10 * some && (a.pairs / Q4_BIG_ITEM + some / 2) * column_blocks >= 512;
     a.item = big ? Q4_BIG_ITEM : Q4_ITEM;

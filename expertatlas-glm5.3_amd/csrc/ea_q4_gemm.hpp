@@ -249,7 +249,8 @@ __device__ __forceinline__ void q4_gemm(uint8_t* lds, const uint8_t* w, uint32_t
             const uint32_t tile0 = (at.cb * 4 + wave) * NT;
             if constexpr (TURN) {  // 16 rows of the wave's columns at a time, where the chunks were once no wave reads them
                 if constexpr (!RESIDENT) __syncthreads();
-                float* const mine = reinterpret_cast<float*>(RESIDENT ? lds_sums + 2 * MT * 1024 : lds) + wave * q4_turn_floats<NT>();
+                float* const mine =
+                    reinterpret_cast<float*>(RESIDENT ? lds_sums + 2 * MT * 1024 : lds) + wave * q4_turn_floats<NT>();
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
                     f4v v[NT];

@@ -176,6 +176,15 @@ def test_gpu_linear_sizes(ea, k, group, n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(17, 1024, 2080), (47, 83, 6144), (256, 256, 2176), (257, 250, 6144), (300, 250, 2048),
+                                   (129, 4200, 2112), (600, 1000, 320), (40, 9000, 256), (16, 9000, 4096), (3, 26000, 2080)])
+def test_gpu_linear_many_blocks(ea, m, n, k):
+    """Rows and columns on both sides of each change of the kernels' form."""
+    _linear(ea, m, k, [n], 32, BF16, BF16, [F32], seed=m)
+    _linear(ea, m, k, [n], 32, F16, F16, [BF16], pad=4)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("k,group", [(32, 32), (320, 64), (1152, 128), (6144, 64)])
 @pytest.mark.parametrize("m", [1, 4, 16, 20, 64, 100, 300])
 def test_gpu_linear_exact_on_integers(ea, m, k, group):
