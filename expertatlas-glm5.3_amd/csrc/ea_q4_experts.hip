@@ -8,7 +8,8 @@
 //
 // A pair takes 6 D I operations, an expert that is picked 3 D I / 2 bytes of words and 12 D I / group of scales and biases: up
 // to some tens of rows the weights' bytes bound it, at one row latencies. Figures in this file: D 6144, I 256, 256 experts,
-// 8 picks a row, groups of 64, bf16 in and out: 1.77 MB gate|up and 0.88 MB down an expert.
+// 8 picks a row (even ones up to 512 rows, Zipf 1.1 above), groups of 64, bf16 in and out: 1.77 MB gate|up and 0.88 MB down an
+// expert.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -455,10 +456,11 @@ __device__ __forceinline__ Q4Place q4_place(const Q4MoeArgs& a, uint32_t blocks)
 }
 static unsigned q4_place_blocks(uint32_t max_items, uint32_t blocks) { return Q4_DIES * (max_items / Q4_DIES + 2) * blocks; }
 
-// Two tiles a wave with more than 32 rows, else four: 2048 rows 265 us (390 TFLOP/s), with four throughout 290. Matrix
-// instructions alone would take a third of that; conversions and scalings hardly overlap them, every operand comes from LDS
-// for two products only, and blocks end unevenly: items of up to 80 or 96 rows, which convert fewer weights, take as long
-// (266, 280) at 2048 rows and longer (206, 218 against 185) at 1024.
+// Two tiles a wave with more than 32 rows, else four: 2048 rows 265 us (390 TFLOP/s), with four throughout 290. Counters have
+// the matrix units busy a fifth of the time and the vector units a third, with 1.3 waves a SIMD on average of the two that
+// the registers allow: waves wait for a chunk's rows, for each other and, at the end, for the last blocks. Items of up to 80
+// or 96 rows, which convert fewer weights, take as long (266, 280) at 2048 rows and longer (206, 218 against 185) at 1024;
+// column blocks side by side in place of one after the other, for the rows' sake, 265 at 2048 and 228 at 1024.
 template <bool BF, bool SBF, int GPC, int NT4, int NT>
 __global__ void __launch_bounds__(Q4_GEMM_THREADS, 2) q4_gateup_gemm_kernel(Q4MoeArgs a, uint32_t blocks) {
     __shared__ __attribute__((aligned(16))) uint8_t lds[std::max(q4_gemm_lds<4, NT4>(), q4_gemm_lds<2, NT>())];

@@ -294,9 +294,9 @@ enum { EA_SCORE_SIGMOID = 0, EA_SCORE_SOFTMAX = 1 };
  * choices are held in 64 bits, so the picks do not depend on how a 32-bit score rounds; wts is rounded once.
  * An expert whose logit is -inf is out: it is never picked, it gives its run nothing, and where fewer than `slots` are left
  * the slots behind get pick -1 and weight 0: a slot without an expert for ea_q4_routed (the EXL3 experts' calls take experts
- * only). A NaN choice ranks below every number, NaNs by the lower expert. 1..EA_ROUTE_MAX_EXPERTS experts, 1..32 slots (EA_TOO_MANY_SLOTS: more, or
- * more than the kept runs hold), 1..64 groups that divide experts (EA_UNEVEN_SPLIT). No counterpart in the reference, whose
- * router is ea_topk8's alone. */
+ * only). A NaN choice ranks below every number, NaNs by the lower expert. 1..EA_ROUTE_MAX_EXPERTS experts, 1..32 slots
+ * (EA_TOO_MANY_SLOTS: more, or more than the kept runs hold), 1..64 groups that divide experts (EA_UNEVEN_SPLIT). No
+ * counterpart in the reference, whose router is ea_topk8's alone. */
 int ea_route(ea_stream_t stream, const void* logits, int l_dtype, uint32_t l_stride, const float* bias, int32_t* pick,
              float* wts, uint32_t rows, uint32_t experts, uint32_t slots, int score, uint32_t groups, uint32_t top_groups,
              uint32_t group_best, int renorm, float scale);
@@ -333,8 +333,8 @@ typedef struct ea_q4_linear {
 int ea_q4_call(ea_stream_t stream, const ea_q4_linear* const* ls, uint32_t nls, const void* x, int x_dtype,
                uint32_t x_stride, uint32_t m, const uint64_t* outs, const int* out_dtypes);
 
-/* One layer's routed experts, 16-byte aligned: gate | up packed together ([count] x ea_q4_bytes(16 * ceil(width / 8), dims, group)) and down
- * ([count] x ea_q4_bytes(dims, width, group)). dims and width are multiples of group; at most 4096 experts. */
+/* One layer's routed experts, 16-byte aligned: gate | up packed together ([count] x ea_q4_bytes(16 * ceil(width / 8), dims,
+ * group)) and down ([count] x ea_q4_bytes(dims, width, group)). dims and width are multiples of group; at most 4096 experts. */
 typedef struct ea_q4_experts {
     uint64_t gu, down;
     uint32_t count, dims, width, group;
@@ -351,9 +351,9 @@ size_t ea_q4_scratch_bytes(const ea_q4_experts* ex, uint32_t rows, uint32_t slot
 int ea_q4_scratch_init(ea_q4_scratch* s, void* base, size_t bytes, const ea_q4_experts* ex, uint32_t rows, uint32_t slots);
 
 /* out [R, dims] (fp16, bf16 or fp32) = sum over the slots of wts * down(silu(gate(x)) * up(x)) of the picked experts: what
- * ea_moe_routed and ea_prompt_experts_run are for EXL3 experts, for one row to a whole prompt's (EA_Q4_MAX_PAIRS). pick int32 / wts fp32
- * [R, slots] (slots: the scratch's); a pick outside 0 .. count - 1 is a slot without an expert, a row of such picks gives
- * zeros, and a row may name an expert twice. The activated values are held as one, two or three bf16 numbers that add up to
+ * ea_moe_routed and ea_prompt_experts_run are for EXL3 experts, for one row to a whole prompt's (EA_Q4_MAX_PAIRS).
+ * pick int32 / wts fp32 [R, slots] (slots: the scratch's); a pick outside 0 .. count - 1 is a slot without an expert, a row
+ * of such picks gives zeros, and a row may name an expert twice. The activated values are held as one, two or three bf16 numbers that add up to
  * them, as many as out's type can show. The same bits on every run. EA_SCRATCH_TOO_SMALL: R above the scratch's rows, or a
  * layer larger than the one it was made for. */
 int ea_q4_routed(ea_stream_t stream, const void* x, int x_dtype, uint32_t x_stride, const int32_t* pick, const float* wts,
