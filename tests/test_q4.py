@@ -382,6 +382,38 @@ def test_gpu_experts_odd_picks(ea, R):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("out_dtype", [BF16, F32])
+def test_gpu_experts_odd_picks_in_long_items(ea, out_dtype):
+    """The same where items are long: rows of NaN between others of their items, an infinite activation, rows without experts,
+    picks outside, an expert named twice."""
+    g = torch.Generator().manual_seed(11)
+    E, D, I, S, R = 6, 192, 512, 3, 1500
+    mats = _layer(g, E, D, I, 64, BF16)
+    x = torch.randn((R, D), generator=g).to(BF16)
+    pick, wts = _routing(g, R, E, S)
+    pick[::7] = torch.tensor([2, -1, 2], dtype=torch.int32)
+    pick[::11] = -1
+    wts[::11], x[::11] = float("nan"), float("nan")
+    pick[5::13, 1] = E
+    wts[5::13, 1] = float("inf")
+    bad = torch.arange(1, R, 37)
+    bad = bad[(bad % 7 != 0) & (bad % 11 != 0)]
+    pick[bad] = torch.tensor([0, 3, 5], dtype=torch.int32)
+    wts[bad] = 0.5
+    x[bad[::2]] = float("nan")
+    x[bad[1::2], 4] = float("inf")
+    out, _, _ = _experts(ea, x, pick, wts, mats, out_dtype)
+    assert not torch.isfinite(out[bad.cuda()]).any()
+    assert (out[::11] == 0).all()
+    live = (pick >= 0) & (pick < E)
+    clean = torch.where(torch.isfinite(x), x, 0)
+    want, err = plain.experts(clean.double(), torch.where(live, pick, -1), torch.where(live, wts, 0), *mats, out_dtype)
+    rest = torch.ones(R, dtype=torch.bool)
+    rest[bad] = False
+    plain.close(out[rest.cuda()], want[rest], err[rest])
+
+
+@pytest.mark.gpu
 def test_gpu_experts_scratch_serves_smaller_calls(ea):
     """A scratch made for more rows and a larger layer, used again and again: the same bits as with one of its own."""
     device, ops, q4 = ea
