@@ -52,7 +52,7 @@ struct Q4MoeArgs {
 // ---- grouping -----------------------------------------------------------------------------------------------------
 // One block: the pairs of each expert counted, the items before each expert scanned, the pairs placed (in any order within an
 // expert). Full items come before all others, so that the longest work starts first. A pick outside 0 .. experts - 1 is a slot
-// without an expert. Bound by its passes' latencies: 5 us at 64 rows, 12 at 512, 15 at 2048 (with items in four classes of
+// without an expert. Bound by its passes' latencies: 5 us at 64 rows, 8 at 512, 15 at 2048 (with items in four classes of
 // size instead of two 24, and 3 % less in the products behind).
 __device__ void q4_group(const Q4MoeArgs& a) {
     __shared__ uint32_t count[Q4_MAX_EXPERTS], full[Q4_MAX_EXPERTS], rest[Q4_MAX_EXPERTS], sums[2][16], all;
@@ -126,18 +126,20 @@ __device__ void q4_group(const Q4MoeArgs& a) {
     }
 }
 
-// The grouping, and with more blocks beside it the rows' sums over groups, a wave a row.
+// The grouping, and with more blocks beside it the rows' sums over groups, four waves a row: with one, whose loads come one
+// after another, both take 12.5 us at 512 rows in place of 8.0.
+constexpr uint32_t Q4_SUM_WAVES = 4;
 __global__ void __launch_bounds__(1024) q4_group_kernel(Q4MoeArgs a) {
     if (blockIdx.x == 0) {
         q4_group(a);
         return;
     }
-    const uint32_t i = (blockIdx.x - 1) * 16 + (threadIdx.x >> 6);
+    const uint32_t w = (blockIdx.x - 1) * 16 + (threadIdx.x >> 6), i = w / Q4_SUM_WAVES, part = w % Q4_SUM_WAVES;
     if (i >= a.rows) return;
     uint8_t* to = a.xsums + (size_t)i * q4_sum_bytes(a.dims / a.group);
     const uint16_t* row = a.x + (size_t)i * a.x_stride;
-    if (a.bf) q4_row_sums<true>(row, 1, 0, a.dims, a.group, to, threadIdx.x & 63);
-    else q4_row_sums<false>(row, 1, 0, a.dims, a.group, to, threadIdx.x & 63);
+    if (a.bf) q4_row_sums<true>(row, 1, 0, a.dims, a.group, to, threadIdx.x & 63, part, Q4_SUM_WAVES);
+    else q4_row_sums<false>(row, 1, 0, a.dims, a.group, to, threadIdx.x & 63, part, Q4_SUM_WAVES);
 }
 
 // The same for up to 16 rows, in the order of the experts' first pairs, by a block beside the first products (picks: the
@@ -413,7 +415,7 @@ __global__ void __launch_bounds__(256) q4_hsums_kernel(Q4MoeArgs a) {
     const uint32_t i = blockIdx.x * 4 + (threadIdx.x >> 6);
     if (i < a.pairs && (uint32_t)a.pick[i] < a.experts)
         q4_row_sums<true>(a.h + (size_t)i * a.width, a.terms, (size_t)a.pairs * a.width, a.width, a.group,
-                          a.hsums + (size_t)i * q4_sum_bytes(a.width / a.group), threadIdx.x & 63);
+                          a.hsums + (size_t)i * q4_sum_bytes(a.width / a.group), threadIdx.x & 63, 0, 1);
 }
 
 // ---- long items -----------------------------------------------------------------------------------------------------
@@ -460,7 +462,8 @@ static unsigned q4_place_blocks(uint32_t max_items, uint32_t blocks) { return Q4
 // the matrix units busy a fifth of the time and the vector units a third, with 1.3 waves a SIMD on average of the two that
 // the registers allow: waves wait for a chunk's rows, for each other and, at the end, for the last blocks. Items of up to 80
 // or 96 rows, which convert fewer weights, take as long (266, 280) at 2048 rows and longer (206, 218 against 185) at 1024;
-// column blocks side by side in place of one after the other, for the rows' sake, 265 at 2048 and 228 at 1024.
+// column blocks side by side in place of one after the other, for the rows' sake, 265 at 2048 and 228 at 1024. At 512 rows
+// 256 experts just fill the card with two blocks each: 113 us, but 157 where one of them has 33 rows and four.
 template <bool BF, bool SBF, int GPC, int NT4, int NT>
 __global__ void __launch_bounds__(Q4_GEMM_THREADS, 2) q4_gateup_gemm_kernel(Q4MoeArgs a, uint32_t blocks) {
     __shared__ __attribute__((aligned(16))) uint8_t lds[std::max(q4_gemm_lds<4, NT4>(), q4_gemm_lds<2, NT>())];
@@ -711,14 +714,14 @@ int ea_q4_routed(ea_stream_t stream, const void* x, int x_dtype, uint32_t x_stri
     a.terms = q4_terms(out_dtype);
     // Long items pay where experts have more than about ten rows each, so that items of 16 would turn most weights twice, and
     // where there are blocks enough to fill the card, as an item's waves no longer share a tile's chunks. All launches with
-    // short / long items: 256 rows 190 / 195 us, 320 201 / 196, 384 220 / 210, 512 279 / 220, 2048 847 / 563.
+    // short / long items: 256 rows 190 / 190 us, 320 201 / 191, 384 220 / 205, 512 279 / 216, 2048 847 / 563.
     const uint64_t some = std::min<uint64_t>(a.pairs, a.experts), column_blocks = ((a.width + 7) / 8 + 7) / 8;
     const bool big = R > Q4_ROWS && a.pairs > 10 * some && (a.pairs / Q4_BIG_ITEM + some / 2) * column_blocks >= 512;
     a.item = big ? Q4_BIG_ITEM : Q4_ITEM;
     const uint32_t max_items = q4_max_items(a.experts, a.pairs, a.item);
     hipStream_t s = as_stream(stream);
     const bool sbf = ex->s_dtype == BF16;
-    if (R > Q4_ROWS) q4_group_kernel<<<1 + (big ? (R + 15) / 16 : 0), 1024, 0, s>>>(a);
+    if (R > Q4_ROWS) q4_group_kernel<<<1 + (big ? (R * Q4_SUM_WAVES + 15) / 16 : 0), 1024, 0, s>>>(a);
     launch_gateup(s, a, x_dtype == BF16, sbf, gpc, max_items);
     if (big) q4_hsums_kernel<<<(a.pairs + 3) / 4, 256, 0, s>>>(a);
     if (a.terms == 1) launch_down<1>(s, a, sbf, gpc, max_items);

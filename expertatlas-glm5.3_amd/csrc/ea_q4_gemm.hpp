@@ -112,12 +112,13 @@ struct Q4Biases {
     }
 };
 
-// A row's sums over its groups, in that form: a wave a row, eight values a lane; `terms` of the row, `plane` values apart.
+// A row's sums over its groups, in that form, by `parts` waves of which this is one, eight values a lane; `terms` of the row,
+// `plane` values apart.
 template <bool BF>
 __device__ __forceinline__ void q4_row_sums(const uint16_t* row, uint32_t terms, size_t plane, uint32_t k, uint32_t group,
-                                            uint8_t* to, int lane) {
+                                            uint8_t* to, int lane, uint32_t part, uint32_t parts) {
     const uint32_t groups = k / group, per = group / 8, padded = (groups + 7) / 8 * 8;
-    for (uint32_t p = lane; p - lane < padded * per; p += 64) {  // a piece of eight values
+    for (uint32_t p = 64 * part + lane; p - lane < padded * per; p += 64 * parts) {  // a piece of eight values
         float v = 0.0f;
         if (p < k / 8)
             for (uint32_t t = 0; t < terms; ++t) {
