@@ -39,7 +39,7 @@ struct Q4MoeArgs {
     size_t gu_bytes, down_bytes;  // one expert's
     int32_t* nitems;              // items, full ones among them
     Q4Item* items;
-    uint16_t* h;                  // bf16 [terms][pairs][width]
+    uint16_t* h;                  // bf16 [terms][pairs][width], terms 2 or 3
     uint8_t *xsums, *hsums;       // sums over groups of a row of x, of a pair of h (q4_row_sums)
     float* y;                     // fp32 [pairs][dims]
     void* out;
@@ -369,7 +369,7 @@ __global__ void __launch_bounds__(64 * WK) q4_down_one_kernel(Q4MoeArgs a) {
 // apart adds the terms. 16 rows 21 us (4.3 TB/s), 64 rows 44 us (4.5 TB/s): the weights, and a pair's fp32 sums, 24 KB each.
 template <bool SBF, int GPC, int TERMS, int NT, int WK, int NB>
 __global__ void __launch_bounds__(64 * WK) q4_down_kernel(Q4MoeArgs a) {
-    constexpr int PER = TERMS == 1 ? 16 : TERMS == 2 ? 8 : 4;  // pairs a product
+    constexpr int PER = TERMS == 2 ? 8 : 4;  // pairs a product
     __shared__ float turn[WK][q4_turn_floats<NT>()];
     const Q4Item& it = a.items[blockIdx.y];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -399,7 +399,7 @@ __global__ void __launch_bounds__(64 * WK) q4_down_kernel(Q4MoeArgs a) {
                 for (int i = 0; i < 4; ++i) {
                     v[t][i] = out[t][i];
                     if constexpr (TERMS == 3) v[t][i] = v[t][i] + lane_xor<16>(v[t][i]);
-                    if constexpr (TERMS >= 2) v[t][i] = v[t][i] + lane_xor<32>(v[t][i]);
+                    v[t][i] = v[t][i] + lane_xor<32>(v[t][i]);
                 }
             q4_turn<NT>(turn[wave], v, lane, [&](int r, int c, const f4v& p) {
                 const uint32_t col = tile0 * 16 + c;
@@ -420,19 +420,37 @@ __global__ void __launch_bounds__(256) q4_hsums_kernel(Q4MoeArgs a) {
 
 // ---- long items -----------------------------------------------------------------------------------------------------
 // An item's products by q4_gemm, with as many row groups as it has: NT4 tiles a wave with four of them, NT with fewer.
-// Column blocks are counted in 4 NT4 tiles; the ones behind the last return.
-template <bool BF, bool SBF, int GPC, int NT4, int NT, bool RESIDENT, bool TURN, typename ROW, typename SUMS, typename STORE>
+// Column blocks are counted in 4 NT4 tiles; the ones behind the last return. Rows of several terms are taken in two halves of
+// the item: with four row groups down takes, at 2048 rows and with two terms, 250 us in place of 224 (groups of 64; 199 and 226
+// with 32, 187 and 213 with 128, but 337 and 224 with fp16 scales, where registers run out), with three 505 in place of 260.
+constexpr int q4_item_groups(int terms) { return terms > 1 ? 2 : 4; }
+template <bool BF, bool SBF, int GPC, int NT4, int NT, int TERMS, bool RESIDENT, bool TURN, typename ROW, typename SUMS,
+          typename STORE>
 __device__ __forceinline__ void q4_item_gemm(uint8_t* lds, int count, const uint8_t* w, uint32_t tiles, uint32_t k,
-                                             uint32_t terms, size_t plane, uint32_t cb, uint32_t cb_step, ROW row,
-                                             SUMS sums, STORE store) {
-    const auto go = [&](auto mt_, auto nt_) __attribute__((always_inline)) {
-        q4_gemm<BF, SBF, GPC, decltype(mt_)::value, decltype(nt_)::value, RESIDENT, TURN>(lds, w, tiles, k, terms, plane, cb,
-                                                                                        cb_step, row, sums, store);
+                                             size_t plane, uint32_t cb, uint32_t cb_step, ROW row, SUMS sums, STORE store) {
+    const auto go = [&](auto mt_, auto nt_, auto r, auto rs, auto st) __attribute__((always_inline)) {
+        q4_gemm<BF, SBF, GPC, decltype(mt_)::value, decltype(nt_)::value, TERMS, RESIDENT, TURN>(lds, w, tiles, k, plane, cb,
+                                                                                               cb_step, r, rs, st);
     };
-    if (count > 32) go(std::integral_constant<int, 4>{}, std::integral_constant<int, NT4>{});
-    else if (cb * 4 * NT >= tiles) return;
-    else if (count > 16) go(std::integral_constant<int, 2>{}, std::integral_constant<int, NT>{});
-    else go(std::integral_constant<int, 1>{}, std::integral_constant<int, NT>{});
+    const std::integral_constant<int, 1> one;
+    const std::integral_constant<int, 2> two;
+    const std::integral_constant<int, NT> nt;
+    if constexpr (q4_item_groups(TERMS) == 2) {
+        static_assert(TURN && NT == NT4);
+        for (int m0 = 0; m0 < count; m0 += 32) {
+            const auto r = [&](int i) { return row(m0 + i); };
+            const auto rs = [&](int i) { return sums(m0 + i); };
+            const auto st = [&](int m, uint32_t col, const f4v& v) { store(m0 + m, col, v); };
+            if (m0) __syncthreads();  // the first half's last readers of LDS
+            if (count - m0 > 16) go(two, nt, r, rs, st);
+            else go(one, nt, r, rs, st);
+        }
+    } else {
+        if (count > 32) go(std::integral_constant<int, 4>{}, std::integral_constant<int, NT4>{}, row, sums, store);
+        else if (cb * 4 * NT >= tiles) return;
+        else if (count > 16) go(two, nt, row, sums, store);
+        else go(one, nt, row, sums, store);
+    }
 }
 
 // Blocks go to the card's eight dies in turn, and each die has an L2 of its own: die x takes the x-th eighth of the full items
@@ -466,14 +484,14 @@ static unsigned q4_place_blocks(uint32_t max_items, uint32_t blocks) { return Q4
 // 256 experts just fill the card with two blocks each: 113 us, but 157 where one of them has 33 rows and four.
 template <bool BF, bool SBF, int GPC, int NT4, int NT>
 __global__ void __launch_bounds__(Q4_GEMM_THREADS, 2) q4_gateup_gemm_kernel(Q4MoeArgs a, uint32_t blocks) {
-    __shared__ __attribute__((aligned(16))) uint8_t lds[std::max(q4_gemm_lds<4, NT4>(), q4_gemm_lds<2, NT>())];
+    __shared__ __attribute__((aligned(16))) uint8_t lds[q4_gemm_lds<4, 1>()];
     const Q4Place at = q4_place(a, blocks);
     if (at.item < 0) return;
     const Q4Item& it = a.items[at.item];
     const int e = it.expert, count = it.count;
     const auto row_of = [&](int i) { return (size_t)((uint32_t)it.pair[min(i, count - 1)] / a.slots); };
-    q4_item_gemm<BF, SBF, GPC, NT4, NT, false, false>(
-        lds, count, a.gu + (size_t)e * a.gu_bytes, (a.width + 7) / 8, a.dims, 1, 0, at.cb, 1u << 24,
+    q4_item_gemm<BF, SBF, GPC, NT4, NT, 1, false, false>(
+        lds, count, a.gu + (size_t)e * a.gu_bytes, (a.width + 7) / 8, a.dims, 0, at.cb, 1u << 24,
         [&](int i) { return a.x + row_of(i) * a.x_stride; },
         [&](int i) { return a.xsums + row_of(i) * q4_sum_bytes(a.dims / a.group); },
         [&](uint32_t tile, const auto& v) {
@@ -493,19 +511,18 @@ __global__ void __launch_bounds__(Q4_GEMM_THREADS, 2) q4_gateup_gemm_kernel(Q4Mo
 }
 
 // A block takes every `blocks`-th column block of an item, six blocks an item at most, and with RESIDENT keeps its rows in LDS
-// meanwhile. 2048 rows 175 us: 403 MB of fp32 sums written and 226 MB of weights read (3.6 TB/s). In two launches of half the
-// columns, each with its sums over slots behind, which then find them in the last-level cache, both together take 266
-// instead of 274 us at 2048 rows, but 183 instead of 157 at 1024.
-template <bool SBF, int GPC, int NT, bool RESIDENT>
+// meanwhile. 2048 rows 224 us with two terms, 259 with three: 403 MB of fp32 sums written and 226 MB of weights read. With a
+// weight turned into an operand once a term in place of once, two terms took 323 us and three 345.
+template <bool SBF, int GPC, int TERMS, int NT, bool RESIDENT>
 __global__ void __launch_bounds__(Q4_GEMM_THREADS, 2) q4_down_gemm_kernel(Q4MoeArgs a, uint32_t blocks) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const Q4Place at = q4_place(a, blocks);
     if (at.item < 0) return;
     const Q4Item& it = a.items[at.item];
     const int e = it.expert, count = it.count;
-    q4_item_gemm<true, SBF, GPC, NT, NT, RESIDENT, true>(
-        lds, count, a.down + (size_t)e * a.down_bytes, q4_tiles(a.dims), a.width, a.terms, (size_t)a.pairs * a.width,
-        at.cb, blocks, [&](int i) { return a.h + (size_t)it.pair[min(i, count - 1)] * a.width; },
+    q4_item_gemm<true, SBF, GPC, NT, NT, TERMS, RESIDENT, true>(
+        lds, count, a.down + (size_t)e * a.down_bytes, q4_tiles(a.dims), a.width, (size_t)a.pairs * a.width, at.cb, blocks,
+        [&](int i) { return a.h + (size_t)it.pair[min(i, count - 1)] * a.width; },
         [&](int i) { return a.hsums + (size_t)it.pair[min(i, count - 1)] * q4_sum_bytes(a.width / a.group); },
         [&](int m, uint32_t col, const f4v& v) {
             if (m < count && col < a.dims) *reinterpret_cast<f4v*>(a.y + (size_t)it.pair[m] * a.dims + col) = v;
@@ -592,22 +609,26 @@ static void launch_down(hipStream_t s, const Q4MoeArgs& a, bool sbf, int gpc, ui
             constexpr int GPC = decltype(gpc_)::value;
             if (a.rows == 1) q4_down_one_kernel<SBF, GPC, TERMS, 1, 8, 2><<<tiles, 512, 0, s>>>(a);
             else if (a.item == Q4_BIG_ITEM) {
-                const uint32_t blocks = std::min((tiles + 15) / 16, 6u), buffers = TERMS * q4_chunks(a.width);
-                const unsigned grid = q4_place_blocks(max_items, blocks);
-                if (buffers <= Q4_RESIDENT)
-                    q4_down_gemm_kernel<SBF, GPC, 4, true>
-                        <<<grid, Q4_GEMM_THREADS, q4_gemm_lds<4, 4>((int)buffers), s>>>(a, blocks);
-                else q4_down_gemm_kernel<SBF, GPC, 4, false><<<grid, Q4_GEMM_THREADS, q4_gemm_lds<4, 4>(), s>>>(a, blocks);
+                constexpr int MT = q4_item_groups(TERMS), NT = 4;
+                const uint32_t chunks = q4_chunks(a.width);
+                const auto blocks = [&](uint32_t nt) { return std::min((tiles + 4 * nt - 1) / (4 * nt), 6u); };
+                if (chunks <= Q4_RESIDENT / (TERMS * MT * 4096))
+                    q4_down_gemm_kernel<SBF, GPC, TERMS, 4, true>
+                        <<<q4_place_blocks(max_items, blocks(4)), Q4_GEMM_THREADS,
+                           q4_gemm_lds<MT, TERMS>((int)chunks, (int)(chunks * GPC + 7) / 8), s>>>(a, blocks(4));
+                else
+                    q4_down_gemm_kernel<SBF, GPC, TERMS, NT, false>
+                        <<<q4_place_blocks(max_items, blocks(NT)), Q4_GEMM_THREADS, q4_gemm_lds<MT, TERMS>(), s>>>(a, blocks(NT));
             } else if (tiles >= 4) q4_down_kernel<SBF, GPC, TERMS, 4, 8, 1><<<dim3((tiles + 31) / 32, max_items), 512, 0, s>>>(a);
             else q4_down_kernel<SBF, GPC, TERMS, 1, 4, 1><<<dim3((tiles + 3) / 4, max_items), 256, 0, s>>>(a);
         }
     });
 }
 
-// Terms of the activated values: what the output's type can show (bf16 8 bits, fp16 11, fp32 24). So with bf16 out h is
-// rounded once, as a layer in bf16 does; a second term would take 2 to 5 % at few rows and, at 2048, the down products from
-// 177 to 368 us.
-static int q4_terms(int out_dtype) { return out_dtype == BF16 ? 1 : out_dtype == F16 ? 2 : 3; }
+// Terms of the activated values: more bits than the output's type can show (bf16 8, fp16 11, fp32 24), so that the output's
+// own rounding is what its error comes from. One term with bf16 out was off by 0.0023 of the output's norm where its rounding
+// is 0.0017, for 0.4 to 1.6 us less of down up to 64 rows and 195 in place of 265 us at 2048.
+static int q4_terms(int out_dtype) { return out_dtype == F32 ? 3 : 2; }
 
 static uint32_t q4_max_items(uint32_t experts, size_t pairs, uint32_t item = Q4_ITEM) {
     const size_t full = pairs / item, some = pairs < experts ? pairs : experts;
@@ -724,8 +745,7 @@ int ea_q4_routed(ea_stream_t stream, const void* x, int x_dtype, uint32_t x_stri
     if (R > Q4_ROWS) q4_group_kernel<<<1 + (big ? (R * Q4_SUM_WAVES + 15) / 16 : 0), 1024, 0, s>>>(a);
     launch_gateup(s, a, x_dtype == BF16, sbf, gpc, max_items);
     if (big) q4_hsums_kernel<<<(a.pairs + 3) / 4, 256, 0, s>>>(a);
-    if (a.terms == 1) launch_down<1>(s, a, sbf, gpc, max_items);
-    else if (a.terms == 2) launch_down<2>(s, a, sbf, gpc, max_items);
+    if (a.terms == 2) launch_down<2>(s, a, sbf, gpc, max_items);
     else launch_down<3>(s, a, sbf, gpc, max_items);
     if (R > 1) q4_combine_kernel<<<dim3(R, (a.dims + 1023) / 1024), 256, 0, s>>>(a);
     return launched();

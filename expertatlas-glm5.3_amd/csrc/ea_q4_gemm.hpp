@@ -9,24 +9,58 @@
 namespace ea {
 
 constexpr int Q4_GEMM_THREADS = 256;
-// LDS: `buffers` chunks of 16 MT rows, 4096 MT bytes each, two buffers of their sums over eight groups, 1024 MT each, and the
-// waves' places to turn their sums: behind them (RESIDENT), or in the place of all.
-template <int MT, int NT>
-constexpr int q4_gemm_lds(int buffers = 0) {
-    const int turn = 4 * 4 * q4_turn_floats<NT>(), two = 2 * MT * (4096 + 1024);
-    return buffers ? buffers * MT * 4096 + 2 * MT * 1024 + turn : two > turn ? two : turn;
+// LDS: chunks of 16 MT rows with all TERMS of the rows, 4096 MT TERMS bytes each (`resident` of them, or two), their sums over
+// eight groups each, 1024 MT bytes (of all groups, or in two buffers), and the waves' places to turn two tiles' sums: behind
+// them, or in the place of all.
+template <int MT, int TERMS>
+constexpr int q4_gemm_lds(int resident = 0, int eights = 2) {
+    const int turn = 4 * 4 * q4_turn_floats<2>(), sums = eights * MT * 1024, two = 2 * MT * 4096 * TERMS + sums;
+    return resident ? resident * MT * 4096 * TERMS + sums + turn : two > turn ? two : turn;
 }
-constexpr int Q4_RESIDENT = 4;  // chunks of all terms that stay in LDS at most
+constexpr int Q4_RESIDENT = 65536;  // bytes of chunks that stay in LDS at most, so that a CU holds two blocks
 
 // One chunk from LDS: row r of the block at 256 r, its 16-byte piece q at 16 (q ^ (r & 15)), so that the 16 rows of an
 // operand's quarter lie in different banks. With BIAS the groups' biases are applied here, from sums of x that are made here
-// too; without, out gets the scaled sums alone.
-template <bool BF, bool SBF, int GPC, int MT, int NT, bool BIAS>
+// too; without, out gets the scaled sums alone. Rows of several TERMS, 4096 MT bytes apart, add up: a weight is turned into an
+// operand once for all of them, and their products share an accumulator.
+template <bool BF, bool SBF, int GPC, int MT, int NT, bool BIAS, int TERMS = 1>
 __device__ __forceinline__ void q4_gemm_chunk(const uint8_t* lds, const u4v (&words)[NT], const Q4Params<GPC> (&par)[NT],
                                               int lane, f4v (&out)[NT][MT]) {
     constexpr int JPG = 4 / GPC;
     const f4v zero{0.0f, 0.0f, 0.0f, 0.0f};
     const int r = lane & 15, quad = lane >> 4;
+    if constexpr (TERMS > 1) {
+        static_assert(!BIAS, "biases of several terms come from their sums");
+#pragma unroll
+        for (int g = 0; g < GPC; ++g) {
+            f4v acc[NT][MT];
+#pragma unroll
+            for (int j = 0; j < JPG; ++j) {
+                u4v b[NT];
+#pragma unroll
+                for (int t = 0; t < NT; ++t) b[t] = q4_values<BF>(words[t][g * JPG + j]);
+#pragma unroll
+                for (int term = 0; term < TERMS; ++term)
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) {
+                        const u4v a = *reinterpret_cast<const u4v*>(lds + ((term * MT + mt) * 16 + r) * 256 +
+                                                                    16 * ((4 * (g * JPG + j) + quad) ^ r));
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) acc[t][mt] = q4_mfma<BF>(a, b[t], j || term ? acc[t][mt] : zero);
+                    }
+            }
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                float s, b;
+                q4_scale_bias<SBF>(par[t].w[g], s, b);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) out[t][mt][i] = __builtin_fmaf(s, acc[t][mt][i], out[t][mt][i]);
+            }
+        }
+        return;
+    }
 #pragma unroll
     for (int g = 0; g < GPC; ++g) {
         u4v a[MT][JPG];
@@ -96,9 +130,12 @@ struct Q4Biases {
             if constexpr (SBF) {
                 shift((w0 >> 16) | (w1 & 0xffff0000u), 0);
             } else {
+                // fp16's 11 bits: the upper 8 as they stand, which leaves 3
                 const float a = h2f((uint16_t)(w0 >> 16)), b = h2f((uint16_t)(w1 >> 16));
-                const uint16_t ah = f2bf(a), bh = f2bf(b);
-                shift((uint32_t)ah | (uint32_t)bh << 16, (uint32_t)f2bf(a - bf2f(ah)) | (uint32_t)f2bf(b - bf2f(bh)) << 16);
+                const uint32_t ah = __builtin_bit_cast(uint32_t, a) & 0xffff0000u, bh = __builtin_bit_cast(uint32_t, b) & 0xffff0000u;
+                const uint32_t al = __builtin_bit_cast(uint32_t, a - __builtin_bit_cast(float, ah));
+                const uint32_t bl = __builtin_bit_cast(uint32_t, b - __builtin_bit_cast(float, bh));
+                shift(ah >> 16 | bh, al >> 16 | (bl & 0xffff0000u));
             }
         }
     }
@@ -147,46 +184,51 @@ __device__ __forceinline__ void q4_row_sums(const uint16_t* row, uint32_t terms,
 }
 
 // The column blocks cb, cb + cb_step, .. of W (its first tile at w) times the block's rows. row(i): row i's activations,
-// terms of them `plane` values apart (their products add up); sums(i): its groups' sums, for the biases. With TURN store(row,
+// TERMS of them `plane` values apart (their products add up); sums(i): its groups' sums, for the biases. With TURN store(row,
 // column of W's packed rows, the sums of four columns), else store(tile, the lane's sums). RESIDENT: all of the rows' terms and
-// chunks lie in LDS at once (Q4_RESIDENT of them at most), so that after the first barrier the waves go on alone; else two
+// chunks lie in LDS at once (Q4_RESIDENT bytes at most), so that after the first barrier the waves go on alone; else two
 // chunks do. Weights are read a chunk before their products.
-template <bool BF, bool SBF, int GPC, int MT, int NT, bool RESIDENT, bool TURN, typename ROW, typename SUMS, typename STORE>
-__device__ __forceinline__ void q4_gemm(uint8_t* lds, const uint8_t* w, uint32_t tiles, uint32_t k, uint32_t terms,
-                                        size_t plane, uint32_t cb, uint32_t cb_step, ROW row, SUMS sums, STORE store) {
+template <bool BF, bool SBF, int GPC, int MT, int NT, int TERMS, bool RESIDENT, bool TURN, typename ROW, typename SUMS,
+          typename STORE>
+__device__ __forceinline__ void q4_gemm(uint8_t* lds, const uint8_t* w, uint32_t tiles, uint32_t k, size_t plane,
+                                        uint32_t cb, uint32_t cb_step, ROW row, SUMS sums, STORE store) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t chunks = q4_chunks(k), piece = threadIdx.x & 15, row0 = threadIdx.x >> 4;
     const uint32_t tile_bytes = chunks * q4_chunk_bytes(GPC);
     constexpr uint32_t CYCLE = 8 / GPC;  // chunks of eight groups
+    constexpr uint32_t BUFFER = TERMS * MT * 4096;
     const uint16_t* src[MT];
 #pragma unroll
     for (int i = 0; i < MT; ++i) src[i] = row(row0 + 16 * i);
     // the sums' 16-byte pieces, one a thread: row threadIdx / 4, piece threadIdx % 4 at 16 (4 row + (piece ^ (row / 4 & 3)))
     const uint32_t srow = threadIdx.x >> 2, sto = 16 * (4 * srow + ((threadIdx.x & 3) ^ (srow >> 2 & 3)));
     const uint8_t* const rs = sums(min(srow, 16u * MT - 1)) + 16 * (threadIdx.x & 3);
-    uint8_t* const lds_sums = lds + (RESIDENT ? terms * chunks : 2) * (MT * 4096);
+    uint8_t* const lds_sums = lds + (RESIDENT ? chunks : 2) * BUFFER;
     const uint32_t to = row0 * 256 + 16 * (piece ^ row0);  // row0 + 16 i: 4096 bytes further each
-    u4v ra[MT], rw[2][NT], rx{};
+    u4v ra[TERMS][MT], rw[2][NT], rx{};
     Q4Params<GPC> rp[2][NT];
     Q4Biases<SBF, GPC> biases[NT];
     struct Cursor {
-        uint32_t cb, term, c;
+        uint32_t cb, c;
     };
     const auto next = [&](Cursor at) {
-        if (++at.c == chunks) at.c = 0, ++at.term;
-        if (at.term == terms) at.term = 0, at.cb += cb_step;
+        if (++at.c == chunks) at.c = 0, at.cb += cb_step;
         return at;
     };
     const auto inside = [&](const Cursor& at) { return at.cb * 4 * NT < tiles; };
-    const auto load_rows = [&](uint32_t term, uint32_t c) {
+    const auto load_rows = [&](uint32_t c) {
         // past k, where the weights are zeros, the row's last 32 values again
         const uint32_t at = c * Q4_CHUNK + 8 * piece, off = at < k ? at : k - 32 + 8 * (piece & 3);
 #pragma unroll
-        for (int i = 0; i < MT; ++i) ra[i] = *reinterpret_cast<const u4v_a8*>(src[i] + term * plane + off);
+        for (int t = 0; t < TERMS; ++t)
+#pragma unroll
+            for (int i = 0; i < MT; ++i) ra[t][i] = *reinterpret_cast<const u4v_a8*>(src[i] + t * plane + off);
     };
     const auto stage = [&](uint32_t buffer) {
 #pragma unroll
-        for (int i = 0; i < MT; ++i) *reinterpret_cast<u4v*>(lds + buffer * (MT * 4096) + to + 4096 * i) = ra[i];
+        for (int t = 0; t < TERMS; ++t)
+#pragma unroll
+            for (int i = 0; i < MT; ++i) *reinterpret_cast<u4v*>(lds + buffer * BUFFER + to + 4096 * (t * MT + i)) = ra[t][i];
     };
     const auto load = [&](int set, const Cursor& at) {
 #pragma unroll
@@ -202,65 +244,62 @@ __device__ __forceinline__ void q4_gemm(uint8_t* lds, const uint8_t* w, uint32_t
     for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) out[t][mt] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
-    Cursor at{cb, 0, 0};
+    Cursor at{cb, 0};
     uint32_t buffer = 0;
     // one chunk; false after the last
     const auto step = [&](auto set_) __attribute__((always_inline)) {
         constexpr int SET = decltype(set_)::value;
-        const uint32_t c = at.c, term = at.term;
+        const uint32_t c = at.c;
         if constexpr (!RESIDENT) stage(buffer);
-        const bool ends = c + 1 == chunks && term + 1 == terms;  // of the column block
+        const bool ends = c + 1 == chunks;  // of the column block
         const Cursor then = next(at);
         const bool more = inside(then);
         // Eight groups' sums are read with the first of their chunks, and go to LDS a chunk later (a barrier after the other
         // buffer's last readers), or at once if no chunk follows: with one chunk in all, over the same values.
-        uint8_t* const cycle_sums = lds_sums + (c / CYCLE & 1) * (MT * 1024);
-        if constexpr (!RESIDENT)
-            if (term == 0) {
-                if (c % CYCLE == 0) rx = *reinterpret_cast<const u4v*>(rs + c / CYCLE * 64);
-                if ((c % CYCLE == 1 || (c % CYCLE == 0 && c + 1 == chunks)) && srow < 16u * MT)
-                    *reinterpret_cast<u4v*>(cycle_sums + sto) = rx;
-            }
-        if constexpr (!RESIDENT)
-            if (more) load_rows(then.term, then.c);
+        uint8_t* const cycle_sums = lds_sums + (RESIDENT ? c / CYCLE : c / CYCLE & 1) * (MT * 1024);
+        if constexpr (!RESIDENT) {
+            if (c % CYCLE == 0) rx = *reinterpret_cast<const u4v*>(rs + c / CYCLE * 64);
+            if ((c % CYCLE == 1 || (c % CYCLE == 0 && ends)) && srow < 16u * MT)
+                *reinterpret_cast<u4v*>(cycle_sums + sto) = rx;
+            if (more) load_rows(then.c);
+        }
         if (more) load(1 - SET, then);
         if constexpr (!RESIDENT) __syncthreads();  // the chunk is staged; its buffer's last readers were before the last one
-        q4_gemm_chunk<BF, SBF, GPC, MT, NT, false>(lds + (RESIDENT ? term * chunks + c : buffer) * (MT * 4096), rw[SET], rp[SET],
-                                                  lane, out);
-        if (term == 0) {
+        q4_gemm_chunk<BF, SBF, GPC, MT, NT, false, TERMS>(lds + (RESIDENT ? c : buffer) * BUFFER, rw[SET], rp[SET], lane, out);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int t = 0; t < NT; ++t) biases[t].take(rp[SET][t]);
-            if (c % CYCLE == CYCLE - 1 || c + 1 == chunks) {
-                for (uint32_t i = c % CYCLE; i < CYCLE - 1; ++i) {  // no more chunks: zeros up to the eighth group
-                    constexpr Q4Params<GPC> none{};
+        for (int t = 0; t < NT; ++t) biases[t].take(rp[SET][t]);
+        if (c % CYCLE == CYCLE - 1 || ends) {
+            for (uint32_t i = c % CYCLE; i < CYCLE - 1; ++i) {  // no more chunks: zeros up to the eighth group
+                constexpr Q4Params<GPC> none{};
 #pragma unroll
-                    for (int t = 0; t < NT; ++t) biases[t].take(none);
-                }
-                u4v a[MT];
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-                    const int r = mt * 16 + (lane & 15);
-                    a[mt] = *reinterpret_cast<const u4v*>(cycle_sums + 16 * (4 * r + ((lane >> 4) ^ (r >> 2 & 3))));
-                }
-#pragma unroll
-                for (int t = 0; t < NT; ++t) biases[t].add(a, out[t]);
+                for (int t = 0; t < NT; ++t) biases[t].take(none);
             }
+            u4v a[MT];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                const int r = mt * 16 + (lane & 15);
+                a[mt] = *reinterpret_cast<const u4v*>(cycle_sums + 16 * (4 * r + ((lane >> 4) ^ (r >> 2 & 3))));
+            }
+#pragma unroll
+            for (int t = 0; t < NT; ++t) biases[t].add(a, out[t]);
         }
         if (ends) {
             const uint32_t tile0 = (at.cb * 4 + wave) * NT;
             if constexpr (TURN) {  // 16 rows of the wave's columns at a time, where the chunks were once no wave reads them
                 if constexpr (!RESIDENT) __syncthreads();
-                float* const mine =
-                    reinterpret_cast<float*>(RESIDENT ? lds_sums + 2 * MT * 1024 : lds) + wave * q4_turn_floats<NT>();
+                static_assert(NT % 2 == 0);
+                float* const mine = reinterpret_cast<float*>(RESIDENT ? lds_sums + (chunks + CYCLE - 1) / CYCLE * (MT * 1024) : lds) +
+                                    wave * q4_turn_floats<2>();
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-                    f4v v[NT];
+                for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                    for (int t = 0; t < NT; ++t) v[t] = out[t][mt];
-                    q4_turn<NT>(mine, v, lane, [&](int r, int c, const f4v& p) {
-                        if (tile0 + c / 16 < tiles) store(16 * mt + r, tile0 * 16 + c, p);
-                    });
-                }
+                    for (int t = 0; t < NT; t += 2) {
+                        const f4v v[2] = {out[t][mt], out[t + 1][mt]};
+                        q4_turn<2>(mine, v, lane, [&](int r, int c, const f4v& p) {
+                            if (tile0 + t + c / 16 < tiles) store(16 * mt + r, (tile0 + t) * 16 + c, p);
+                        });
+                    }
                 if constexpr (!RESIDENT)
                     if (more) __syncthreads();
             } else {
@@ -277,14 +316,13 @@ __device__ __forceinline__ void q4_gemm(uint8_t* lds, const uint8_t* w, uint32_t
         buffer ^= 1;
         return more;
     };
-    if constexpr (!RESIDENT) load_rows(0, 0);
+    if constexpr (!RESIDENT) load_rows(0);
     load(0, at);
     if constexpr (RESIDENT) {
-        for (uint32_t t = 0; t < terms; ++t)
-            for (uint32_t ci = 0; ci < chunks; ++ci) {
-                load_rows(t, ci);
-                stage(t * chunks + ci);
-            }
+        for (uint32_t ci = 0; ci < chunks; ++ci) {
+            load_rows(ci);
+            stage(ci);
+        }
         for (uint32_t i = 0; i * CYCLE < chunks; ++i)
             if (srow < 16u * MT)
                 *reinterpret_cast<u4v*>(lds_sums + i * (MT * 1024) + sto) = *reinterpret_cast<const u4v*>(rs + i * 64);

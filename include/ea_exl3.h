@@ -353,9 +353,9 @@ int ea_q4_scratch_init(ea_q4_scratch* s, void* base, size_t bytes, const ea_q4_e
 /* out [R, dims] (fp16, bf16 or fp32) = sum over the slots of wts * down(silu(gate(x)) * up(x)) of the picked experts: what
  * ea_moe_routed and ea_prompt_experts_run are for EXL3 experts, for one row to a whole prompt's (EA_Q4_MAX_PAIRS).
  * pick int32 / wts fp32 [R, slots] (slots: the scratch's); a pick outside 0 .. count - 1 is a slot without an expert, a row
- * of such picks gives zeros, and a row may name an expert twice. The activated values are held as one, two or three bf16 numbers that add up to
- * them, as many as out's type can show. The same bits on every run. EA_SCRATCH_TOO_SMALL: R above the scratch's rows, or a
- * layer larger than the one it was made for. */
+ * of such picks gives zeros, and a row may name an expert twice. The activated values are held as two bf16 numbers that add up
+ * to them (16 bits), with fp32 out as three (24 bits). The same bits on every run. EA_SCRATCH_TOO_SMALL: R above the
+ * scratch's rows, or a layer larger than the one it was made for. */
 int ea_q4_routed(ea_stream_t stream, const void* x, int x_dtype, uint32_t x_stride, const int32_t* pick, const float* wts,
                  const ea_q4_experts* ex, const ea_q4_scratch* s, void* out, int out_dtype, uint32_t R);
 
