@@ -88,14 +88,13 @@ __global__ void __launch_bounds__(64 * WK) q4_linear_kernel(Q4LinArgs a) {
     const uint32_t tiles = q4_tiles(job.n), tile0 = blockIdx.x * NT;
     if (tile0 >= tiles) return;
     const size_t tile_bytes = (size_t)a.chunks * q4_chunk_bytes(GPC);
-    const uint32_t first = min(tile0, tiles - min(tiles, (uint32_t)NT));  // the last block's tiles overlap
+    const uint32_t own = min(tiles, (uint32_t)NT), first = min(tile0, tiles - own);  // the last block's tiles overlap
     const uint32_t m0 = blockIdx.y * 16, m = min(a.m - m0, 16u);
     const uint16_t* row = a.x + (size_t)(m0 + min((uint32_t)(lane & 15), m - 1)) * a.x_stride;  // past m the last row again
     f4v out[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) out[t] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
-    q4_stream<BF, SBF, GPC, NT, NB>(job.w + first * tile_bytes, tiles < NT ? 0 : tile_bytes, wave, WK, a.chunks, row, a.k, lane,
-                                    out);
+    q4_stream<BF, SBF, GPC, NT, NB>(job.w + first * tile_bytes, tile_bytes, wave, WK, a.chunks, row, a.k, lane, out, own - 1);
 #pragma unroll
     for (int t = 0; t < NT; ++t) part[wave][t][lane] = out[t];
     __syncthreads();

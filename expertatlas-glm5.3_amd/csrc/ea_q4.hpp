@@ -108,11 +108,13 @@ __device__ __forceinline__ void q4_rows(const uint16_t* row, uint32_t chunk, uin
     for (int j = 0; j < 4; ++j) a[j] = (u4v) * reinterpret_cast<const u4v_a8*>(p + min(32 * j, last));
 }
 
-// The tiles at w, w + tile_bytes, .. against 16 rows over the chunks c0, c0 + step, ..: the loads of NB chunks are issued
-// before the first of their products. With SOME, a lane whose row is null reads nothing and multiplies zeros.
+// The tiles at w, w + tile_bytes, .. (of a matrix with fewer than NT the last one again) against 16 rows over the chunks c0,
+// c0 + step, ..: the loads of NB chunks are issued before the first of their products. With SOME, a lane whose row is null
+// reads nothing and multiplies zeros.
 template <bool BF, bool SBF, int GPC, int NT, int NB, bool SOME = false>
 __device__ __forceinline__ void q4_stream(const uint8_t* w, size_t tile_bytes, uint32_t c0, uint32_t step, uint32_t chunks,
-                                          const uint16_t* row, uint32_t k, int lane, f4v (&out)[NT]) {
+                                          const uint16_t* row, uint32_t k, int lane, f4v (&out)[NT],
+                                          uint32_t last_tile = NT - 1) {
     for (uint32_t c = c0; c < chunks; c += step * NB) {
         u4v words[NB][NT], x[NB][4];
         Q4Params<GPC> par[NB][NT];
@@ -121,7 +123,7 @@ __device__ __forceinline__ void q4_stream(const uint8_t* w, size_t tile_bytes, u
             const uint32_t ci = min(c + step * i, chunks - 1);
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                const uint8_t* p = w + t * tile_bytes + (size_t)ci * q4_chunk_bytes(GPC);
+                const uint8_t* p = w + min((uint32_t)t, last_tile) * tile_bytes + (size_t)ci * q4_chunk_bytes(GPC);
                 words[i][t] = reinterpret_cast<const u4v*>(p)[lane];
                 par[i][t] = q4_params<GPC>(p, lane);
             }
