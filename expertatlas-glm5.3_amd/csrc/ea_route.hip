@@ -77,8 +77,9 @@ __device__ __forceinline__ void wave_fence() {
 }
 
 // 1 / (1 + exp(-x)) in 64 bits: v_rcp_f64's estimate and two Newton steps (an IEEE division takes twice the instructions).
+// Below -709.7827 exp(-x) is no number any more: scores end at that one's, 5.6e-309.
 __device__ __forceinline__ double sigmoid64(double x) {
-    const double d = 1.0 + exp(__builtin_fmin(-x, 709.0));
+    const double d = 1.0 + exp(__builtin_fmin(-x, 709.7827));
     double r = __builtin_amdgcn_rcp(d);
     r = __builtin_fma(r, __builtin_fma(-d, r, 1.0), r);
     r = __builtin_fma(r, __builtin_fma(-d, r, 1.0), r);
