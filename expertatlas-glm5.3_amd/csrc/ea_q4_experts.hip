@@ -20,6 +20,8 @@
 
 namespace ea {
 
+// dims and width are multiples of a group, so of 32 (q4_experts_ok): gate|up has width / 8 tiles, four or more, down dims / 16,
+// two or more, none of them with rows behind its matrix.
 constexpr uint32_t Q4_MAX_EXPERTS = 4096;
 constexpr uint32_t Q4_ITEM = 16, Q4_BIG_ITEM = 64;         // pairs an item
 constexpr uint32_t Q4_ROWS = 16, Q4_PAIRS = Q4_ROWS * 32;  // rows and pairs that are grouped beside the first products
@@ -223,7 +225,7 @@ __global__ void __launch_bounds__(64 * WK) q4_gateup_kernel(Q4MoeArgs a) {
     __shared__ f4v part[WK][NT][64];
     __shared__ int32_t picks[MODE == FEW_ROWS ? Q4_PAIRS : 16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t u = blockIdx.y, chunks = q4_chunks(a.dims), tiles = (a.width + 7) / 8, r = lane & 15;
+    const uint32_t u = blockIdx.y, chunks = q4_chunks(a.dims), r = lane & 15;
     int32_t e;
     const uint16_t* row = nullptr;
     int count = 0;
@@ -255,7 +257,7 @@ __global__ void __launch_bounds__(64 * WK) q4_gateup_kernel(Q4MoeArgs a) {
         if (threadIdx.x < 16) picks[r] = p;
         if ((int)r < count) row = a.x + (size_t)((uint32_t)p / a.slots) * a.x_stride;
     }
-    const uint32_t tile0 = min(blockIdx.x * NT, tiles - NT);  // the last block's tiles overlap
+    const uint32_t tile0 = blockIdx.x * NT;
     const size_t tile_bytes = (size_t)chunks * q4_chunk_bytes(GPC);
     f4v out[NT];
 #pragma unroll
@@ -269,17 +271,17 @@ __global__ void __launch_bounds__(64 * WK) q4_gateup_kernel(Q4MoeArgs a) {
         const int n = i & 7, t = (i >> 3) % NT, m = i / (8 * NT);
         const uint32_t col = (tile0 + t) * 8 + n;
         uint32_t p = u;
-        bool is = col < a.width;
-        if constexpr (MODE == ONE_ROW) is = is && m == 0;
+        bool is = true;
+        if constexpr (MODE == ONE_ROW) is = m == 0;
         if constexpr (MODE == FEW_ROWS) {  // the row's first naming of the expert
             p = m * a.slots;
             const uint32_t end = (uint32_t)m < a.rows ? p + a.slots : p;
             while (p < end && picks[p] != e) ++p;
-            is = is && p < end;
+            is = p < end;
         }
         if constexpr (MODE == ITEMS) {
             p = picks[m];
-            is = is && m < count;
+            is = m < count;
         }
         if (!is) continue;
         const float v = swiglu(q4_total<WK, NT>(part, t, m, n), q4_total<WK, NT>(part, t, m, n + 8));
@@ -295,8 +297,8 @@ template <bool SBF, int GPC, int TERMS, int NT, int WK, int NB>
 __global__ void __launch_bounds__(64 * WK) q4_down_one_kernel(Q4MoeArgs a) {
     __shared__ f4v part[WK][NT][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), term = lane & 15;
-    const uint32_t chunks = q4_chunks(a.width), tiles = q4_tiles(a.dims), units = a.slots * chunks;
-    const uint32_t tile0 = min(blockIdx.x * NT, tiles - NT);
+    const uint32_t chunks = q4_chunks(a.width), units = a.slots * chunks;
+    const uint32_t tile0 = blockIdx.x * NT;
     const size_t tile_bytes = (size_t)chunks * q4_chunk_bytes(GPC), plane = (size_t)a.slots * a.width;
     f4v out[NT];
 #pragma unroll
@@ -353,12 +355,10 @@ __global__ void __launch_bounds__(64 * WK) q4_down_one_kernel(Q4MoeArgs a) {
     __syncthreads();
     for (int i = threadIdx.x; i < 16 * NT; i += 64 * WK) {
         const int n = i & 15, t = i >> 4;
-        const uint32_t col = (tile0 + t) * 16 + n;
-        if (col >= a.dims) continue;
         float v = q4_total<WK, NT>(part, t, TERMS - 1, n);
 #pragma unroll
         for (int r = TERMS - 2; r >= 0; --r) v = v + q4_total<WK, NT>(part, t, r, n);  // the small terms first
-        store_act(a.out, a.out_dtype, col, v);
+        store_act(a.out, a.out_dtype, (tile0 + t) * 16 + n, v);
     }
 }
 
@@ -402,9 +402,8 @@ __global__ void __launch_bounds__(64 * WK) q4_down_kernel(Q4MoeArgs a) {
                     v[t][i] = v[t][i] + lane_xor<32>(v[t][i]);
                 }
             q4_turn<NT>(turn[wave], v, lane, [&](int r, int c, const f4v& p) {
-                const uint32_t col = tile0 * 16 + c;
-                if (r < PER && m0 + r < count && col < a.dims)
-                    *reinterpret_cast<f4v*>(a.y + (size_t)it.pair[m0 + r] * a.dims + col) = p;
+                if (r < PER && m0 + r < count)
+                    *reinterpret_cast<f4v*>(a.y + (size_t)it.pair[m0 + r] * a.dims + tile0 * 16 + c) = p;
             });
         }
     }
@@ -491,7 +490,7 @@ __global__ void __launch_bounds__(Q4_GEMM_THREADS, 2) q4_gateup_gemm_kernel(Q4Mo
     const int e = it.expert, count = it.count;
     const auto row_of = [&](int i) { return (size_t)((uint32_t)it.pair[min(i, count - 1)] / a.slots); };
     q4_item_gemm<BF, SBF, GPC, NT4, NT, 1, false, false>(
-        lds, count, a.gu + (size_t)e * a.gu_bytes, (a.width + 7) / 8, a.dims, 0, at.cb, 1u << 24,
+        lds, count, a.gu + (size_t)e * a.gu_bytes, a.width / 8, a.dims, 0, at.cb, 1u << 24,
         [&](int i) { return a.x + row_of(i) * a.x_stride; },
         [&](int i) { return a.xsums + row_of(i) * q4_sum_bytes(a.dims / a.group); },
         [&](uint32_t tile, const auto& v) {
@@ -503,7 +502,7 @@ __global__ void __launch_bounds__(Q4_GEMM_THREADS, 2) q4_gateup_gemm_kernel(Q4Mo
                 for (int i = 0; i < 4; ++i) {
                     const float u = lane_xor<8>(v[mt][i]);  // lanes 0 .. 7 of 16 have the gate, the others the up column
                     const int m = 16 * mt + 4 * (lane >> 4) + i;
-                    if ((lane & 8) || m >= count || col >= a.width) continue;
+                    if ((lane & 8) || m >= count) continue;
                     store_terms(a.h, a.terms, (size_t)a.pairs * a.width, (size_t)it.pair[m] * a.width + col,
                                 swiglu(v[mt][i], u));
                 }
@@ -525,7 +524,7 @@ __global__ void __launch_bounds__(Q4_GEMM_THREADS, 2) q4_down_gemm_kernel(Q4MoeA
         [&](int i) { return a.h + (size_t)it.pair[min(i, count - 1)] * a.width; },
         [&](int i) { return a.hsums + (size_t)it.pair[min(i, count - 1)] * q4_sum_bytes(a.width / a.group); },
         [&](int m, uint32_t col, const f4v& v) {
-            if (m < count && col < a.dims) *reinterpret_cast<f4v*>(a.y + (size_t)it.pair[m] * a.dims + col) = v;
+            if (m < count) *reinterpret_cast<f4v*>(a.y + (size_t)it.pair[m] * a.dims + col) = v;
         });
 }
 
@@ -582,21 +581,18 @@ __global__ void __launch_bounds__(256) q4_combine_kernel(Q4MoeArgs a) {
 
 // ---- launches -------------------------------------------------------------------------------------------------------
 static void launch_gateup(hipStream_t s, const Q4MoeArgs& a, bool bf, bool sbf, int gpc, uint32_t max_items) {
-    const uint32_t tiles = (a.width + 7) / 8;
+    const uint32_t tiles = a.width / 8;
     q4_types(bf, sbf, gpc, [&](auto gpc_, auto bf_, auto sbf_) {
         constexpr bool BF = decltype(bf_)::value, SBF = decltype(sbf_)::value;
         constexpr int GPC = decltype(gpc_)::value;
-        const dim3 one(tiles, a.pairs + (a.rows > 1)), two((tiles + 1) / 2, a.pairs + 1);
-        const bool few = a.rows <= Q4_ROWS;
-        if (a.rows == 1) q4_gateup_kernel<BF, SBF, GPC, 1, 8, 3, ONE_ROW><<<one, 512, 0, s>>>(a);
-        else if (few && tiles < 2) q4_gateup_kernel<BF, SBF, GPC, 1, 8, 3, FEW_ROWS><<<one, 512, 0, s>>>(a);
-        else if (few) q4_gateup_kernel<BF, SBF, GPC, 2, 8, 3, FEW_ROWS><<<two, 512, 0, s>>>(a);
+        if (a.rows == 1) q4_gateup_kernel<BF, SBF, GPC, 1, 8, 3, ONE_ROW><<<dim3(tiles, a.pairs), 512, 0, s>>>(a);
+        else if (a.rows <= Q4_ROWS)
+            q4_gateup_kernel<BF, SBF, GPC, 2, 8, 3, FEW_ROWS><<<dim3(tiles / 2, a.pairs + 1), 512, 0, s>>>(a);
         else if (a.item == Q4_BIG_ITEM) {
             const uint32_t blocks = (tiles + 7) / 8;
             const unsigned grid = q4_place_blocks(max_items, blocks);
             q4_gateup_gemm_kernel<BF, SBF, GPC, 2, 4><<<grid, Q4_GEMM_THREADS, 0, s>>>(a, blocks);
-        } else if (tiles < 2) q4_gateup_kernel<BF, SBF, GPC, 1, 8, 3, ITEMS><<<dim3(1, max_items), 512, 0, s>>>(a);
-        else q4_gateup_kernel<BF, SBF, GPC, 2, 8, 3, ITEMS><<<dim3((tiles + 1) / 2, max_items), 512, 0, s>>>(a);
+        } else q4_gateup_kernel<BF, SBF, GPC, 2, 8, 3, ITEMS><<<dim3(tiles / 2, max_items), 512, 0, s>>>(a);
     });
 }
 
@@ -714,7 +710,7 @@ int ea_q4_routed(ea_stream_t stream, const void* x, int x_dtype, uint32_t x_stri
     a.wts = wts;
     a.gu = dptr<const uint8_t>(ex->gu);
     a.down = dptr<const uint8_t>(ex->down);
-    a.gu_bytes = (size_t)((ex->width + 7) / 8) * q4_chunks(ex->dims) * q4_chunk_bytes(gpc);
+    a.gu_bytes = (size_t)(ex->width / 8) * q4_chunks(ex->dims) * q4_chunk_bytes(gpc);
     a.down_bytes = (size_t)q4_tiles(ex->dims) * q4_chunks(ex->width) * q4_chunk_bytes(gpc);
     a.nitems = dptr<int32_t>(sc->count);
     a.items = dptr<Q4Item>(sc->items);
@@ -736,7 +732,7 @@ int ea_q4_routed(ea_stream_t stream, const void* x, int x_dtype, uint32_t x_stri
     // Long items pay where experts have more than about ten rows each, so that items of 16 would turn most weights twice, and
     // where there are blocks enough to fill the card, as an item's waves no longer share a tile's chunks. All launches with
     // short / long items: 256 rows 190 / 190 us, 320 201 / 191, 384 220 / 205, 512 279 / 216, 2048 847 / 563.
-    const uint64_t some = std::min<uint64_t>(a.pairs, a.experts), column_blocks = ((a.width + 7) / 8 + 7) / 8;
+    const uint64_t some = std::min<uint64_t>(a.pairs, a.experts), column_blocks = (a.width / 8 + 7) / 8;
     const bool big = R > Q4_ROWS && a.pairs > 10 * some && (a.pairs / Q4_BIG_ITEM + some / 2) * column_blocks >= 512;
     a.item = big ? Q4_BIG_ITEM : Q4_ITEM;
     const uint32_t max_items = q4_max_items(a.experts, a.pairs, a.item);

@@ -39,17 +39,15 @@ template <int CTL>
 __device__ __forceinline__ uint32_t dpp(uint32_t v) {
     return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTL, 0xf, 0xf, true);
 }
-// f over the L = 16, 32 or 64 lanes of a row: every lane ends with the result (f commutative and associative).
+// f over the L = 32 or 64 lanes of a row: every lane ends with the result (f commutative and associative).
 template <int L, typename F>
 __device__ __forceinline__ uint32_t row_all(uint32_t v, F f) {
     v = f(v, dpp<0xB1>(v));   // quad_perm 1,0,3,2
     v = f(v, dpp<0x4E>(v));   // quad_perm 2,3,0,1
     v = f(v, dpp<0x141>(v));  // row_half_mirror
     v = f(v, dpp<0x140>(v));  // row_mirror
-    if constexpr (L >= 32) {
-        const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-        v = f((uint32_t)a[0], (uint32_t)a[1]);
-    }
+    const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = f((uint32_t)a[0], (uint32_t)a[1]);
     if constexpr (L == 64) {
         const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
         v = f((uint32_t)b[0], (uint32_t)b[1]);
@@ -91,7 +89,7 @@ __device__ __forceinline__ double sigmoid64(double x) {
 // in turn, a row's largest key found by its upper half first, which only ties to 20 bits follow with the lower half and the
 // expert's number. A wave a row has the shortest chain; 32 lanes a row share the steps over the lanes between two rows, which
 // pays when every SIMD has several waves anyway. 256 experts, 8 slots, kernel times, 64 and 32 lanes: 1 row 4.6 us, 512 rows
-// 5.3 and 6.7, 2048 rows 6.2 and 6.8, 4096 rows 8.4 and 7.8 (16 lanes: 9.8 at any of these). The loads of a row had been
+// 5.3 and 6.7, 2048 rows 6.2 and 6.8, 4096 rows 8.4 and 7.8 (16 lanes took 9.8 at any of these). The loads of a row had been
 // behind conditions, waited for one by one: 1 row 5.6 us, 4096 rows 12.3 then.
 template <int EPL, int L, bool GROUPS>
 __global__ void __launch_bounds__(256) route_kernel(RouteArgs a) {
@@ -127,7 +125,6 @@ __global__ void __launch_bounds__(256) route_kernel(RouteArgs a) {
         for (int j = 0; j < EPL; ++j) x[j] = l + L * j < a.experts ? x[j] : -__builtin_inff();
     }
     got[w][l % 32] = -1;
-    if (L < 32) got[w][l + L] = -1;
     double m = 0.0, part = 0.0;
     if (a.softmax) {
         uint32_t top = 0;
