@@ -307,7 +307,7 @@ int ea_route(ea_stream_t stream, const void* logits, int l_dtype, uint32_t l_str
  * consecutive k: the affine format of the reference's draft model (q4.zig, qmm_group.cu) and of checkpoints that are not
  * EXL3-encoded. The products take x as it is (fp16 or bf16), multiply by the integers q and apply scale and bias to fp32
  * sums of a group, so no weight is rounded; a group's bias times its sum of x is added apart, so a row with an infinity
- * gives infinities or NaN in all of its outputs. */
+ * gives infinities or NaN in all of its outputs, and bf16 values from 2^117 on can take a group's sum of q x out of fp32. */
 #define EA_Q4_MAX_ROWS 65536    /* of a linear's call */
 #define EA_Q4_MAX_PAIRS 524288  /* rows * slots of the experts' */
 

@@ -23,16 +23,32 @@ def _ints(gen, shape, group, lo, hi, bias, scale, s_dtype):
     return words, s, torch.full_like(s, bias * scale)
 
 
-def _case(seed, E, D, I, group, slots, R, s_dtype, out_dtype):
+LOUD = slice(8, 16)  # columns of x, and what they hold: 8 bits each, their sum 19
+LOUD_X = torch.tensor([255 * 256, 253 * 256, 191 * 256, 129 * 256, 251 * 128, 247 * 64, 243 * 32, 239 * 16])
+
+
+def _fill(m, columns, q):
+    """The integers of some columns, in whole words, set to q."""
+    words = m[0].clone()
+    words[..., columns.start // 8:columns.stop // 8] = sum(q << (4 * i) for i in range(8)) - (2**32 if q >= 8 else 0)
+    return words, m[1], m[2]
+
+
+def _case(seed, E, D, I, group, slots, R, s_dtype, out_dtype, loud=False):
     """x in 0 .. 2, gate sums large and positive (silu(g) = g there: 1 + exp(-g) is 1 from g = 18 on), up sums of either sign
     in a few of the columns and zero in the others; down weights -1, 0 and 1 over 256. With fp32 out the activated values have up
-    to 20 bits, else up to 14."""
+    to 20 bits, else up to 14. With `loud`, half of the rows have eight large columns, whose weights are zero: s (sum of q x)
+    and b (sum of x) cancel there, numbers of 19 bits and more."""
     g = torch.Generator().manual_seed(seed)
     wide = out_dtype == F32
     x = torch.randint(0, 3, (R, D), generator=g) * (torch.rand((R, D), generator=g) < (64 if wide else 160) / D)
     x[:, ::max(1, D // 32)] = 1  # no row's gate sum is small
-    gate = _ints(g, (E, I, D), group, 0, 15 if wide else 1, 1, 1.0, s_dtype)
+    gate = _ints(g, (E, I, D), group, 2, 15 if wide else 3, -1, 1.0, s_dtype) if loud else \
+        _ints(g, (E, I, D), group, 0, 15 if wide else 1, 1, 1.0, s_dtype)
     up = _ints(g, (E, I, D), group, 0, 14 if wide else 2, -7 if wide else -1, 1.0, s_dtype)
+    if loud:
+        x[::2, LOUD] = LOUD_X
+        gate, up = _fill(gate, LOUD, 1), _fill(up, LOUD, 7 if wide else 1)
     up_zero = torch.ones(I, dtype=torch.bool)
     live = 4 if wide else 16
     up_zero[torch.arange(live) * I // live] = False
@@ -115,3 +131,61 @@ def test_gpu_experts_exact_on_integers(ea, shape, s_dtype, out_dtype):  # noqa: 
     assert low >= 18 and size < 2**24
     out, _, _ = _experts(ea, x, pick, wts, mats, out_dtype, pad=4)
     assert torch.equal(out.cpu(), want.float().to(out_dtype))
+
+
+@pytest.mark.parametrize("shape", [s for s in SHAPES if s[-1] <= 40])
+@pytest.mark.parametrize("s_dtype", [BF16, F16])
+def test_loud_columns_need_every_term(shape, s_dtype):
+    """The sums of x over the loud columns' group are exact in fp32 and need all three bf16 terms (of some row, where there are several)."""
+    for out_dtype in (BF16, F32):
+        x, pick, wts, mats = _case(_seed(shape), *shape, s_dtype, out_dtype, True)
+        _, low, _, size = _plain(x, pick, wts, mats)
+        assert low >= 18 and size < 2**24
+        sums = x[::2, :shape[3]].double().sum(1)
+        assert float(sums.max()) * 15 < 2**24
+        two = sums.float().to(BF16).double()
+        two = two + (sums - two).float().to(BF16).double()
+        assert (two != sums).any() or len(sums) < 2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("s_dtype", [BF16, F16])
+@pytest.mark.parametrize("out_dtype", [BF16, F32])
+def test_gpu_experts_exact_beside_loud_columns(ea, shape, s_dtype, out_dtype):  # noqa: F811
+    """Biases times sums of x that are far larger than what is left: every bit of the sums counts."""
+    x, pick, wts, mats = _case(_seed(shape), *shape, s_dtype, out_dtype, True)
+    want, low, _, size = _plain(x, pick, wts, mats)
+    assert low >= 18 and size < 2**24
+    out, _, _ = _experts(ea, x, pick, wts, mats, out_dtype)
+    assert torch.equal(out.cpu(), want.float().to(out_dtype))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 16, 40, 300])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_gpu_linear_exact_beside_loud_columns(ea, m, dtype):  # noqa: F811
+    device, _, q4 = ea
+    g = torch.Generator().manual_seed(m)
+    w = _fill(_ints(g, (83, 2112), 64, 0, 15, -7, 1.0, dtype), LOUD, 7)
+    x = torch.randint(-3, 4, (m, 2112), generator=g)
+    x[::2, LOUD] = LOUD_X
+    x = x.to(dtype)
+    out, dx = torch.zeros((m, 83), device="cuda"), x.cuda()
+    q4.call(device.stream(), [q4.Linear(*_cuda(w))], dx.data_ptr(), {F16: 0, BF16: 1}[dtype], 2112, m, [out.data_ptr()], [2])
+    assert torch.equal(out.cpu().double(), x.double() @ plain.dense(*w).t())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 16, 40, 300])
+@pytest.mark.parametrize("group", [32, 128])
+def test_gpu_linear_exact_on_the_largest_rows(ea, m, group):  # noqa: F811
+    """bf16 rows up to 2^116, where a group's sum of q x still is a number: 15 x 128 x 2^116 < 2^127."""
+    device, _, q4 = ea
+    g = torch.Generator().manual_seed(m + group)
+    w = _ints(g, (83, 1152), group, 0, 15, -7, 2.0**-20, BF16)
+    x = (torch.randint(-1, 2, (m, 1152), generator=g) * 2.0**116).to(BF16)
+    x[0], w[0][0] = 2.0**116, -1  # the largest sum: q = 15 throughout
+    out, dx = torch.zeros((m, 83), device="cuda"), x.cuda()
+    q4.call(device.stream(), [q4.Linear(*_cuda(w))], dx.data_ptr(), 1, 1152, m, [out.data_ptr()], [2])
+    assert torch.equal(out.cpu().double(), x.double() @ plain.dense(*w).t())
