@@ -729,11 +729,12 @@ int ea_q4_routed(ea_stream_t stream, const void* x, int x_dtype, uint32_t x_stri
     a.slots = sc->slots;
     a.out_dtype = out_dtype;
     a.terms = q4_terms(out_dtype);
-    // Long items pay where experts have more than about ten rows each, so that items of 16 would turn most weights twice, and
-    // where there are blocks enough to fill the card, as an item's waves no longer share a tile's chunks. All launches with
-    // short / long items: 256 rows 190 / 190 us, 320 201 / 191, 384 220 / 205, 512 279 / 216, 2048 847 / 563.
+    // Long items pay where experts have more than about seven rows each (down's short items turn a weight once for every eight
+    // rows of two terms, or four of three) and where there are blocks enough to fill the card, as an item's waves no longer share
+    // a tile's chunks. All launches with short / long items, bf16 out: 128 rows 162 / 174 us, 256 201 / 187, 320 226 / 201, 384
+    // 252 / 212, 512 320 / 229, 2048 960 / 598; fp32 out: 320 265 / 208, 2048 1196 / 614.
     const uint64_t some = std::min<uint64_t>(a.pairs, a.experts), column_blocks = (a.width / 8 + 7) / 8;
-    const bool big = R > Q4_ROWS && a.pairs > 10 * some && (a.pairs / Q4_BIG_ITEM + some / 2) * column_blocks >= 512;
+    const bool big = R > Q4_ROWS && a.pairs > 7 * some && (a.pairs / Q4_BIG_ITEM + some / 2) * column_blocks >= 512;
     a.item = big ? Q4_BIG_ITEM : Q4_ITEM;
     const uint32_t max_items = q4_max_items(a.experts, a.pairs, a.item);
     hipStream_t s = as_stream(stream);
