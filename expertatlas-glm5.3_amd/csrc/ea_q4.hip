@@ -107,11 +107,12 @@ __global__ void __launch_bounds__(64 * WK) q4_linear_kernel(Q4LinArgs a) {
 // More rows: a block takes 16 MT rows and 4 NT tiles, and KS groups of four waves every KS-th chunk of them: each group stages
 // its chunk's rows in LDS, in two buffers, while the chunk before is multiplied, and reads its weights a chunk ahead; the
 // groups' sums are added in order at the end. Four groups of one tile a wave where that makes at most 256 blocks, else two of
-// two tiles: 128 rows x 2048 x 6144 15.4 against 24.8 us, 64 x 8192 x 2048 8.7 against 11.8, but 128 x 6144 x 2048 13.7
-// against 12.5, 301 x 6144 x 2048 26.5 against 19 (400 TFLOP/s). Matrix and vector instructions hardly overlap here
-// (measured: a product takes 17 cycles, a vector instruction 2.4 to 4.5, and together their sum), so waves count more than
-// large tiles: 512 rows x 12000 x 8192 take 189 us with 32 rows, two tiles and two groups, 198 with 64 rows, 212 without
-// groups.
+// two tiles: 128 rows x 2048 x 6144 15.5 against 24.8 us, 64 x 8192 x 2048 8.7 against 11.8, but 128 x 6144 x 2048 13.7
+// against 12.5, 301 x 6144 x 2048 26.5 against 18 (420 TFLOP/s). Bound by the instructions beside the products of rows and
+// weights: the rows' sums are products against ones in every wave, a third of its matrix instructions with two tiles and
+// half with one, and conversions, scales and biases take the vector units. Waves count more than large tiles: 512 rows x
+// 12000 x 8192 took 189 us with 32 rows, two tiles and two groups, 198 with 64 rows, 212 without groups (196 to 240 us for the
+// first of these from one run to the next).
 template <bool BF, bool SBF, int GPC, int MT, int NT, int KS>
 __global__ void __launch_bounds__(256 * KS) q4_linear_split_kernel(Q4LinArgs a) {
     constexpr int BUFFER = MT * 4096, PARTS = KS * 4 * NT * MT * 1024;

@@ -292,7 +292,7 @@ __global__ void __launch_bounds__(64 * WK) q4_gateup_kernel(Q4MoeArgs a) {
 // ---- down -----------------------------------------------------------------------------------------------------------
 // One row: NT tiles of the output a block; its waves take the (slot, chunk) units in turn, weigh their sums in registers, and
 // terms (rows 0 .. TERMS - 1 of the instruction) and waves are added at the end: nothing is left for a launch behind.
-// 4.6 us (1.5 TB/s): the launch, picks, weights and sums after each other.
+// 4.9 us (1.4 TB/s): the launch, picks, weights and sums after each other.
 template <bool SBF, int GPC, int TERMS, int NT, int WK, int NB>
 __global__ void __launch_bounds__(64 * WK) q4_down_one_kernel(Q4MoeArgs a) {
     __shared__ f4v part[WK][NT][64];
@@ -366,7 +366,7 @@ __global__ void __launch_bounds__(64 * WK) q4_down_one_kernel(Q4MoeArgs a) {
 // expert's weights are read where they lie together (blocks that took some tiles of every expert read them at half the rate).
 // Terms are rows of their own: rows 4 q .. 4 q + 3 of the instruction are quad q of the accumulators' lanes; with three
 // terms quad q holds term q of four pairs, with two quads 2 q and 2 q + 1 term q of eight, and adding lanes 16 (and 32)
-// apart adds the terms. 16 rows 21 us (4.3 TB/s), 64 rows 44 us (4.5 TB/s): the weights, and a pair's fp32 sums, 24 KB each.
+// apart adds the terms. 16 rows 24 us (3.8 TB/s), 64 rows 46 us (4.3 TB/s): the weights, and a pair's fp32 sums, 24 KB each.
 template <bool SBF, int GPC, int TERMS, int NT, int WK, int NB>
 __global__ void __launch_bounds__(64 * WK) q4_down_kernel(Q4MoeArgs a) {
     constexpr int PER = TERMS == 2 ? 8 : 4;  // pairs a product
@@ -475,12 +475,13 @@ __device__ __forceinline__ Q4Place q4_place(const Q4MoeArgs& a, uint32_t blocks)
 }
 static unsigned q4_place_blocks(uint32_t max_items, uint32_t blocks) { return Q4_DIES * (max_items / Q4_DIES + 2) * blocks; }
 
-// Two tiles a wave with more than 32 rows, else four: 2048 rows 265 us (390 TFLOP/s), with four throughout 290. Counters have
-// the matrix units busy a fifth of the time and the vector units a third, with 1.3 waves a SIMD on average of the two that
-// the registers allow: waves wait for a chunk's rows, for each other and, at the end, for the last blocks. Items of up to 80
-// or 96 rows, which convert fewer weights, take as long (266, 280) at 2048 rows and longer (206, 218 against 185) at 1024;
-// column blocks side by side in place of one after the other, for the rows' sake, 265 at 2048 and 228 at 1024. At 512 rows
-// 256 experts just fill the card with two blocks each: 113 us, but 157 where one of them has 33 rows and four.
+// Two tiles a wave with more than 32 rows, else four: 2048 rows 265 us (390 TFLOP/s; 254 to 300 by the draw of the routing),
+// with four throughout 290. Counters have the matrix units busy a fifth of the time and the vector units a third, with 1.4
+// waves a SIMD on average of the two that the registers allow: waves wait for a chunk's rows, for each other and, at the end,
+// for the last blocks. Items of up to 80 or 96 rows, which convert fewer weights, take as long (266, 280) at 2048 rows and
+// longer (206, 218 against 185) at 1024; column blocks side by side in place of one after the other, for the rows' sake, 265 at
+// 2048 and 228 at 1024. At 512 rows 256 experts just fill the card with two blocks each: 113 us, but 157 where one of them has
+// 33 rows and four.
 template <bool BF, bool SBF, int GPC, int NT4, int NT>
 __global__ void __launch_bounds__(Q4_GEMM_THREADS, 2) q4_gateup_gemm_kernel(Q4MoeArgs a, uint32_t blocks) {
     __shared__ __attribute__((aligned(16))) uint8_t lds[q4_gemm_lds<4, 1>()];
@@ -510,7 +511,7 @@ __global__ void __launch_bounds__(Q4_GEMM_THREADS, 2) q4_gateup_gemm_kernel(Q4Mo
 }
 
 // A block takes every `blocks`-th column block of an item, six blocks an item at most, and with RESIDENT keeps its rows in LDS
-// meanwhile. 2048 rows 224 us with two terms, 259 with three: 403 MB of fp32 sums written and 226 MB of weights read. With a
+// meanwhile. 2048 rows 224 us with two terms, 249 with three: 403 MB of fp32 sums written and 226 MB of weights read. With a
 // weight turned into an operand once a term in place of once, two terms took 323 us and three 345.
 template <bool SBF, int GPC, int TERMS, int NT, bool RESIDENT>
 __global__ void __launch_bounds__(Q4_GEMM_THREADS, 2) q4_down_gemm_kernel(Q4MoeArgs a, uint32_t blocks) {
@@ -529,7 +530,7 @@ __global__ void __launch_bounds__(Q4_GEMM_THREADS, 2) q4_down_gemm_kernel(Q4MoeA
 }
 
 // ---- a row's slots, in order ----------------------------------------------------------------------------------------
-// Bound by the pairs' sums: 64 rows 5 us (12.6 MB), 2048 rows 85 to 98 us (403 MB read, 25 MB written: 5.0 to 4.4 TB/s).
+// Bound by the pairs' sums: 64 rows 6.5 us (12.6 MB), 2048 rows 94 us (403 MB read, 25 MB written: 4.6 TB/s).
 __global__ void __launch_bounds__(256) q4_combine_kernel(Q4MoeArgs a) {
     __shared__ int32_t pick[32];
     __shared__ float weight[32];

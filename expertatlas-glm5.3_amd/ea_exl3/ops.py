@@ -26,7 +26,7 @@ def route(stream: int, logits: int, l_dtype: int, l_stride: int, bias: int, pick
     """topk for other routers: pick int32 / wts fp32 [rows, slots] from logits [rows, experts] (l_dtype 0 fp16, 1 bf16, 2
     fp32; rows l_stride apart) by sigmoid or softmax scores, a bias (0: none) for the choice, the top_groups best of `groups`
     runs of experts (ranked by their one or two best choices), weights renormalised and scaled. Experts with a logit of -inf
-    are never picked; slots that find no expert get -1 and 0."""
+    are never picked; slots that find no expert get -1 and 0. For topk's own router topk is the faster call."""
     check(lib().ea_route(stream, logits, l_dtype, l_stride, bias, pick, wts, rows, experts, slots, score, groups, top_groups,
                          group_best, int(renorm), scale), "route")
 

@@ -296,7 +296,8 @@ enum { EA_SCORE_SIGMOID = 0, EA_SCORE_SOFTMAX = 1 };
  * the slots behind get pick -1 and weight 0: a slot without an expert for ea_q4_routed (the EXL3 experts' calls take experts
  * only). A NaN choice ranks below every number, NaNs by the lower expert. 1..EA_ROUTE_MAX_EXPERTS experts, 1..32 slots
  * (EA_TOO_MANY_SLOTS: more, or more than the kept runs hold), 1..64 groups that divide experts (EA_UNEVEN_SPLIT). No
- * counterpart in the reference, whose router is ea_topk8's alone. */
+ * counterpart in the reference, whose router is ea_topk8's alone; for that one router ea_topk8, whose scores are in 32 bits, is
+ * the faster call (kernels at 1 / 4096 rows 3.3 / 6.0 us against 4.4 / 7.9). */
 int ea_route(ea_stream_t stream, const void* logits, int l_dtype, uint32_t l_stride, const float* bias, int32_t* pick,
              float* wts, uint32_t rows, uint32_t experts, uint32_t slots, int score, uint32_t groups, uint32_t top_groups,
              uint32_t group_best, int renorm, float scale);
